@@ -238,6 +238,47 @@ typedef struct incin_attn_desc {
 int incin_flash_attn_fwd(const incin_attn_desc* desc, void* stream);
 int incin_flash_attn_bwd(const incin_attn_desc* desc, void* stream);
 
+/* ---- paged key-value cache (serving; no backward) ------------------------------------------------- */
+/* One layer of a cache is k_pages / v_pages [pages, Hkv, page_size, D] (own strides in elements for pages, heads and
+ * tokens, D contiguous; bases 16-byte aligned, strides multiples of 8); page_size is 16, 32, 64 or 128, D is 64 or 128,
+ * dtype INCIN_GEMM_IN_BF16 or INCIN_GEMM_IN_FP16.  Position j of sequence s is slot j % page_size of page
+ * table[s * table_stride + j / page_size] (table_width entries a sequence; entries behind the last token are not read).
+ * lengths[s] counts the tokens of the sequence with its new ones.  The new tokens of all sequences are packed rows:
+ * sequence s has rows [offsets[s], offsets[s + 1]), its last row is its last token; offsets == NULL: one row a sequence.
+ * table, lengths and offsets are read on the device, so a captured launch follows their contents.  A length beyond the
+ * table or an entry outside [0, pages) that is met writes KernelStatus 6 to *status; the entry reads as zeros and is not
+ * written through.  Outputs of rows outside every sequence, and of sequences without tokens, are zeros.
+ * Hq is a multiple of Hkv, Hq / Hkv at most 128. */
+typedef struct incin_paged_desc {
+  void *k_pages, *v_pages;
+  long long k_stride_page, k_stride_head, k_stride_token;
+  long long v_stride_page, v_stride_head, v_stride_token;
+  const int32_t* table;
+  long long table_stride;
+  const int32_t *lengths, *offsets;
+  int table_width, seqs, rows, pages, page_size, Hq, Hkv, D, dtype;
+  float scale;
+  const void* x; /* attention: queries [rows, Hq, D]; append: projections [rows, Hq + 2 Hkv, D] */
+  long long x_stride_row, x_stride_head;
+  void* out; /* dense [rows, Hq, D] */
+  void* workspace; /* 16-byte aligned, as many bytes as the operation's _workspace function says; may be NULL for 0 */
+  void* status;
+} incin_paged_desc;
+/* Rotates queries and keys of the new rows to their positions (rotate-half pairs, theta > 0; 0 leaves them as they are),
+ * writes keys and values into the cache and the queries to out. */
+int incin_kv_append(const incin_paged_desc* desc, double theta, void* stream);
+/* Attention of one new token per sequence (offsets unused, rows == seqs) over its cached tokens. */
+long long incin_decode_attention_workspace(const incin_paged_desc* desc);
+int incin_decode_attention(const incin_paged_desc* desc, void* stream);
+/* Causal attention of packed runs of new tokens over the cached tokens of their sequences. */
+long long incin_prompt_attention_workspace(const incin_paged_desc* desc);
+int incin_prompt_attention(const incin_paged_desc* desc, void* stream);
+/* storage: `outer` runs of `pages` pages of page_bytes (a multiple of 16) each; page dst[i] becomes a copy of page src[i]
+ * in every run.  A pair with an index outside [0, pages), or whose destination is an earlier pair's destination or any
+ * other pair's source, is left out and reported through *status (KernelStatus 6); dst[i] == src[i] copies nothing. */
+int incin_copy_pages(void* storage, const int32_t* src, const int32_t* dst, int pairs, long long outer, int pages,
+                     long long page_bytes, void* status, void* stream);
+
 /* ---- tensor-parallel helpers -------------------------------------------------------------------- */
 /* out[r][n] = sum_s slots[s][r][n] (+ residual[r][n]) in fp32, written as bf16; slots: bf16 [world][rows][ld] */
 int incin_slot_reduce(const void* slots, long long slot_stride, int world, const void* residual, void* out,

@@ -90,6 +90,15 @@ class Block(nn.Module):
         return F.mlp(h, self.fc_w, self.fc_b, self.out_w, self.out_b, act="gelu", residual=res,
                      defer_b2_grad=defer_out_bias)
 
+    def extend(self, x, batch, layer: int):
+        """:meth:`forward` for the packed new tokens ``[1, rows, d_model]`` of a cached batch (no gradients)."""
+        cfg = self.cfg
+        res, h = F.layernorm_fork(x, self.ln1_g, self.ln1_b, cfg.ln_eps)
+        a = batch.attend(layer, F.linear(h, self.qkv_w, self.qkv_b)[0], cfg.n_head)[None]
+        x = F.linear(a, self.proj_w, self.proj_b, residual=res)
+        res, h = F.layernorm_fork(x, self.ln2_g, self.ln2_b, cfg.ln_eps)
+        return F.mlp(h, self.fc_w, self.fc_b, self.out_w, self.out_b, act="gelu", residual=res)
+
 
 class GPT2(nn.Module):
     def __init__(self, cfg: GPT2Config, seed: int = 0):
@@ -128,3 +137,15 @@ class GPT2(nn.Module):
         if targets is None:
             return F.linear(h, self.wte)[..., : cfg.vocab_size]   # tied LM head over the padded vocabulary
         return F.linear_cross_entropy(h, self.wte, targets, cfg.vocab_size)
+
+    @torch.no_grad()
+    def extend(self, tokens, cache, seqs, counts=None):
+        """Append new tokens to cached sequences and return the logits ``[len(seqs), vocab]`` of each one's last token (see
+        :meth:`incin_b200.models.llama.Llama.extend`)."""
+        cfg = self.cfg
+        batch = cache.admit(tokens, seqs, counts, cfg.max_seq)
+        x = F.embedding(tokens[None], self.wte) + F.embedding(batch.positions()[None], self.wpe)
+        for i, b in enumerate(self.blocks):
+            x = b.extend(x, batch, i)
+        h = F.layer_norm(x[0, batch.last_rows()], self.lnf_g, self.lnf_b, cfg.ln_eps)
+        return F.linear(h, self.wte)[..., : cfg.vocab_size]

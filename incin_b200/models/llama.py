@@ -89,6 +89,16 @@ class LlamaBlock(nn.Module):
         g = F.swiglu(F.linear(h, self.gate_up_w))
         return F.linear(g, self.down_w, residual=res)
 
+    def extend(self, x, batch, layer: int):
+        """:meth:`forward` for the packed new tokens ``[1, rows, d_model]`` of a cached batch (no gradients)."""
+        cfg = self.cfg
+        res, h = F.rmsnorm_fork(x, self.attn_norm, cfg.rms_eps)
+        a = batch.attend(layer, F.linear(h, self.qkv_w)[0], cfg.n_head, cfg.rope_theta)[None]
+        x = F.linear(a, self.o_w, residual=res)
+        res, h = F.rmsnorm_fork(x, self.ffn_norm, cfg.rms_eps)
+        g = F.swiglu(F.linear(h, self.gate_up_w))
+        return F.linear(g, self.down_w, residual=res)
+
 
 class Llama(nn.Module):
     def __init__(self, cfg: LlamaConfig, seed: int = 0):
@@ -116,3 +126,15 @@ class Llama(nn.Module):
         if targets is None:
             return F.linear(h, self.lm_head)
         return F.linear_cross_entropy(h, self.lm_head, targets, cfg.vocab_size)
+
+    @torch.no_grad()
+    def extend(self, tokens, cache, seqs, counts=None):
+        """Append new tokens to cached sequences and return the logits ``[len(seqs), vocab]`` of each one's last token.
+        ``tokens`` ``[rows]``: ``counts[i]`` (default 1, at least 1) tokens of sequence ``seqs[i]`` of ``cache``
+        (:class:`~incin_b200.cache.PagedCache`), sequence after sequence."""
+        batch = cache.admit(tokens, seqs, counts, self.cfg.max_seq)
+        x = F.embedding(tokens[None], self.embed, None)
+        for i, b in enumerate(self.blocks):
+            x = b.extend(x, batch, i)
+        h = F.rms_norm(x[0, batch.last_rows()], self.final_norm, self.cfg.rms_eps)
+        return F.linear(h, self.lm_head)

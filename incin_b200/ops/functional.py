@@ -678,3 +678,7 @@ def gqa_attention(qkv, n_heads: int, n_kv_heads: int, head_dim: int, scale: floa
             return A.flash_attention_packed(qkv, n_heads, head_dim, scale, n_kv_heads)
         raise nat.NativeError("no attention kernel for this head configuration (head_dim must be 64 or 128)")
     return _gqa_cpu(qkv, n_heads, n_kv_heads, head_dim, scale)
+
+
+# --------------------------------------------------------------------------------------------- serving from a paged cache
+from .paged import copy_pages, decode_attention, kv_append, prompt_attention  # noqa: E402,F401

@@ -1,0 +1,297 @@
+"""Serving from a paged key-value cache: writing it, attention over it, copying its pages — Python front ends.
+
+One layer of a cache is a pair of tensors ``k_pages``, ``v_pages`` of shape ``[pages, kv_heads, page_size, head_dim]`` (views
+with contiguous rows do).  Position ``j`` of sequence ``s`` lives in page ``table[s, j // page_size]`` at slot ``j % page_size``;
+``lengths[s]`` counts the tokens of the sequence with its new ones.  The new tokens of all sequences are packed rows: those of
+sequence ``s`` are rows ``offsets[s] .. offsets[s + 1]``, and they are its last tokens.  ``table``, ``lengths`` and ``offsets``
+are int32 tensors that are read on the device: no call synchronises, and a captured one follows their contents.  Entries of
+``table`` behind a sequence's last token and slots behind it are never read.  Rows outside every sequence, and sequences without
+tokens, give zeros.
+
+On CUDA the tensors are bf16 or fp16 with head_dim 64 or 128, else the call is refused; the CPU takes any float type.  An
+entry of ``table`` that names no page, or a length that the table cannot hold, raises on the CPU; on CUDA it is met on the
+device: the entry reads as zeros, is not written through, and ``ops.gemm.check_status`` raises.
+
+None of these operators has a backward pass: they refuse inputs that want a gradient.  :class:`incin_b200.cache.PagedCache`
+keeps the tables.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from .. import _native as nat
+from .gemm import status_word
+
+c_void_p, c_int, c_ll, c_float, c_double = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_double
+
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+class PagedDesc(C.Structure):
+    _fields_ = (
+        [("k_pages", c_void_p), ("v_pages", c_void_p)]
+        + [(f"{n}_stride_{a}", c_ll) for n in ("k", "v") for a in ("page", "head", "token")]
+        + [("table", c_void_p), ("table_stride", c_ll), ("lengths", c_void_p), ("offsets", c_void_p),
+           ("table_width", c_int), ("seqs", c_int), ("rows", c_int), ("pages", c_int), ("page_size", c_int),
+           ("Hq", c_int), ("Hkv", c_int), ("D", c_int), ("dtype", c_int), ("scale", c_float),
+           ("x", c_void_p), ("x_stride_row", c_ll), ("x_stride_head", c_ll),
+           ("out", c_void_p), ("workspace", c_void_p), ("status", c_void_p)]
+    )
+
+
+nat.register_cuda_signatures({
+    "incin_kv_append": (c_int, [C.POINTER(PagedDesc), c_double, c_void_p]),
+    "incin_decode_attention_workspace": (c_ll, [C.POINTER(PagedDesc)]),
+    "incin_decode_attention": (c_int, [C.POINTER(PagedDesc), c_void_p]),
+    "incin_prompt_attention_workspace": (c_ll, [C.POINTER(PagedDesc)]),
+    "incin_prompt_attention": (c_int, [C.POINTER(PagedDesc), c_void_p]),
+    "incin_copy_pages": (c_int, [c_void_p] * 3 + [c_int, c_ll, c_int, c_ll, c_void_p, c_void_p]),
+})
+
+_KIND = {torch.bfloat16: nat.GEMM_IN_BF16, torch.float16: nat.GEMM_IN_FP16}
+
+
+# ------------------------------------------------------------------------------------------------------------- checks
+def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int) -> None:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"{what}: k_pages and v_pages must both be [pages, kv_heads, page_size, head_dim], got "
+                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    pages, hkv, size, D = k_pages.shape
+    if size not in PAGE_SIZES:
+        raise ValueError(f"{what}: page_size must be one of {PAGE_SIZES}, got {size}")
+    if not (x.dtype == k_pages.dtype == v_pages.dtype and x.dtype.is_floating_point):
+        raise ValueError(f"{what}: rows and pages must have one float type, got {x.dtype}, {k_pages.dtype} and {v_pages.dtype}")
+    if pages == 0 or hkv == 0 or n_heads <= 0 or n_heads % hkv:
+        raise ValueError(f"{what}: {n_heads} query heads do not fall into {hkv} key heads ({pages} pages)")
+    if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != lengths.shape[0] or table.shape[0] == 0 or table.shape[1] == 0:
+        raise ValueError(f"{what}: table must be [sequences, entries] and lengths [sequences], got {tuple(table.shape)} and "
+                         f"{tuple(lengths.shape)}")
+    seqs = table.shape[0]
+    if offsets is None:
+        if rows != seqs:
+            raise ValueError(f"{what}: {rows} rows for {seqs} sequences (one row each, or offsets)")
+    elif offsets.dim() != 1 or offsets.shape[0] != seqs + 1:
+        raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
+    for name, t in (("table", table), ("lengths", lengths), ("offsets", offsets)):
+        if t is not None and (t.dtype != torch.int32 or t.stride(-1) != 1):
+            raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
+    for t in (k_pages, v_pages, table, lengths, offsets):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if x.is_cuda:
+        if x.dtype not in _KIND or D not in (64, 128):
+            raise nat.NativeError(f"{what}: no kernel for {x.dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
+        if n_heads // hkv > 128:
+            raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+                raise nat.NativeError(f"{what}: {name} needs contiguous rows that start on 16-byte boundaries, got strides {t.stride()}")
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with contiguous heads that start on 16-byte boundaries."""
+    if x.stride(-1) == 1 and not any(s % 8 for s in x.stride()[:-1]) and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _launch(fn, what: str, x, k_pages, v_pages, table, lengths, offsets, n_heads: int, out, scale: float = 0.0, args=(), workspace=None):
+    pages, hkv, size, D = k_pages.shape
+    d = PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], *v_pages.stride()[:3], table.data_ptr(),
+                  table.stride(0), lengths.data_ptr(), nat.ptr(offsets), table.shape[1], table.shape[0], x.shape[0], pages, size,
+                  n_heads, hkv, D, _KIND[x.dtype], scale, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), None,
+                  status_word(x.device).data_ptr())
+    room = None
+    if workspace is not None:
+        n = workspace(C.byref(d))
+        if n:   # of this call alone: two captured graphs share none
+            room = torch.empty(n, dtype=torch.uint8, device=x.device)
+            d.workspace = room.data_ptr()
+    nat.check(fn(C.byref(d), *args, nat.stream_ptr()), what)
+    return out
+
+
+def _on(t: torch.Tensor):
+    """The device of ``t`` made current where it is another one."""
+    return torch.cuda.device(t.device)
+
+
+def _is_current(t: torch.Tensor) -> bool:
+    return t.device.index == torch.cuda.current_device()
+
+
+# ------------------------------------------------------------------------------------------------------------- append
+def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: int, theta: float | None = None):
+    """Write the keys and values of new tokens into the cache and return their queries ``[rows, n_heads, head_dim]``.
+
+    ``qkv``: packed projections ``[rows, (n_heads + 2 kv_heads) * head_dim]`` (query heads first, then key heads, then value
+    heads).  With ``theta`` queries and keys are rotated to their positions first (rotate-half pairs, as
+    :func:`~incin_b200.ops.functional.rope`).  ``offsets=None``: one new token per sequence; a sequence of length 0 is then an
+    idle slot of the batch.  No two new tokens may share a slot."""
+    if k_pages.dim() != 4 or qkv.dim() != 2:
+        raise ValueError(f"kv_append: qkv must be [rows, width] and k_pages [pages, kv_heads, page_size, head_dim], got "
+                         f"{tuple(qkv.shape)} and {tuple(k_pages.shape)}")
+    rows, hkv, D = qkv.shape[0], k_pages.shape[1], k_pages.shape[3]
+    if qkv.shape[1] != (n_heads + 2 * hkv) * D or D % 2:
+        raise ValueError(f"kv_append: rows of {qkv.shape[1]} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
+    if theta is not None and not 1.0 <= theta < 1e300:
+        raise ValueError(f"kv_append: theta must be at least 1, got {theta}")
+    _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    x = qkv.unflatten(1, (n_heads + 2 * hkv, D))
+    if not qkv.is_cuda:
+        return _append_cpu(x, k_pages, v_pages, table, lengths, offsets, n_heads, theta)
+    if not _is_current(qkv):
+        with _on(qkv):
+            return kv_append(qkv, k_pages, v_pages, table, lengths, offsets, n_heads=n_heads, theta=theta)
+    q = torch.empty(rows, n_heads, D, dtype=qkv.dtype, device=qkv.device)
+    if rows == 0:
+        return q
+    return _launch(nat.cuda().incin_kv_append, "kv_append", _rows16(x), k_pages, v_pages, table, lengths, offsets, n_heads, q,
+                   args=(theta or 0.0,))
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+def decode_attention(q, k_pages, v_pages, table, lengths, *, scale: float | None = None):
+    """Attention of one new token per sequence over all its cached tokens: ``q`` ``[sequences, heads, head_dim]`` -> the same
+    shape.  Grouped heads as in :func:`~incin_b200.ops.functional.gqa_attention`; ``scale`` defaults to head_dim^-1/2."""
+    return _attend("decode_attention", q, k_pages, v_pages, table, lengths, None, scale)
+
+
+def prompt_attention(q, k_pages, v_pages, table, lengths, offsets, *, scale: float | None = None):
+    """Causal attention of packed runs of new tokens over the cached tokens of their sequences: ``q``
+    ``[rows, heads, head_dim]`` -> the same shape.  The new tokens' own keys and values are in the cache already
+    (:func:`kv_append`); new token ``i`` of ``n`` sees the first ``lengths[s] - n + i + 1`` positions."""
+    if offsets is None:
+        raise ValueError("prompt_attention: offsets are required (decode_attention takes one row per sequence)")
+    return _attend("prompt_attention", q, k_pages, v_pages, table, lengths, offsets, scale)
+
+
+def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
+    if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3]:
+        raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(q.shape)} and pages "
+                         f"{tuple(k_pages.shape)}")
+    rows, n_heads, D = q.shape
+    _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale) or scale < 0:
+        raise ValueError(f"{what}: scale must be finite and not negative, got {scale}")
+    if not q.is_cuda:
+        return _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale)
+    if not _is_current(q):
+        with _on(q):
+            return _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale)
+    out = torch.empty(rows, n_heads, D, dtype=q.dtype, device=q.device)
+    if rows == 0:
+        return out
+    lib = nat.cuda()
+    fn, room = ((lib.incin_decode_attention, lib.incin_decode_attention_workspace) if offsets is None else
+                (lib.incin_prompt_attention, lib.incin_prompt_attention_workspace))
+    return _launch(fn, what, _rows16(q), k_pages, v_pages, table, lengths, offsets, n_heads, out, scale, workspace=room)
+
+
+# -------------------------------------------------------------------------------------------------------------- pages
+def copy_pages(storage, src, dst):
+    """``storage[..., dst[i], :, :, :] = storage[..., src[i], :, :, :]`` for every pair ``i`` and all leading indices (layers,
+    keys and values), in place; returns ``storage``.  ``storage``: dense ``[..., pages, kv_heads, page_size, head_dim]`` of any
+    type whose pages are multiples of 16 bytes; ``src``, ``dst``: int32 ``[pairs]`` on its device.  A source may be named many
+    times; a destination must be named once and be nobody's source (a page may be its own copy).  Pairs that break this, or
+    name no page, raise on the CPU; on CUDA they are left out and reported through ``ops.gemm.check_status``, the earliest of
+    several equal destinations being kept."""
+    if storage.dim() < 4 or not storage.is_contiguous():
+        raise ValueError(f"copy_pages: storage must be dense [..., pages, kv_heads, page_size, head_dim], got {tuple(storage.shape)}, "
+                         f"strides {storage.stride()}")
+    if src.dim() != 1 or src.shape != dst.shape or src.dtype != torch.int32 or dst.dtype != torch.int32:
+        raise ValueError(f"copy_pages: src and dst must be int32 [pairs], got {tuple(src.shape)} {src.dtype} and {tuple(dst.shape)} {dst.dtype}")
+    if src.device != storage.device or dst.device != storage.device:
+        raise ValueError(f"copy_pages: tensors on {storage.device}, {src.device} and {dst.device}")
+    if torch.is_grad_enabled() and storage.requires_grad:
+        raise RuntimeError("copy_pages has no backward pass: call it under torch.no_grad()")
+    pages = storage.shape[-4]
+    page_bytes = math.prod(storage.shape[-3:]) * storage.element_size()
+    outer = math.prod(storage.shape[:-4])
+    if page_bytes % 16:
+        raise ValueError(f"copy_pages: pages of {page_bytes} bytes, not a multiple of 16")
+    if not storage.is_cuda:
+        a, b = src.tolist(), dst.tolist()
+        moves = [(i, j) for i, j in zip(a, b) if i != j]
+        if any(not 0 <= i < pages for i in a + b):
+            raise IndexError(f"copy_pages: page outside [0, {pages})")
+        if len(set(b)) != len(b) or any(j in a for _, j in moves):
+            raise IndexError("copy_pages: a destination is named twice or is also a source")
+        if moves:
+            flat = storage.view(outer, pages, -1)
+            flat[:, [j for _, j in moves]] = flat[:, [i for i, _ in moves]]
+        return storage
+    if src.numel() == 0 or storage.numel() == 0:
+        return storage
+    if storage.data_ptr() % 16:
+        raise nat.NativeError("copy_pages: storage must start on a 16-byte boundary")
+    if not _is_current(storage):
+        with _on(storage):
+            return copy_pages(storage, src, dst)
+    src, dst = src.contiguous(), dst.contiguous()
+    nat.check(nat.cuda().incin_copy_pages(storage.data_ptr(), src.data_ptr(), dst.data_ptr(), src.numel(), outer, pages, page_bytes,
+                                          status_word(storage.device).data_ptr(), nat.stream_ptr()), "copy_pages")
+    return storage
+
+
+# ----------------------------------------------------------------------------------------------------------- CPU twins
+def _runs(k_pages, table, lengths, offsets, rows):
+    """``(sequence, first row, new tokens, length)`` of every sequence, checked."""
+    size = k_pages.shape[2]
+    lens = lengths.tolist()
+    offs = list(range(rows + 1)) if offsets is None else offsets.tolist()
+    out = []
+    for s, n in enumerate(lens):
+        if not 0 <= n <= table.shape[1] * size:
+            raise IndexError(f"sequence {s}: length {n}, its table holds {table.shape[1] * size}")
+        used = table[s, :(n + size - 1) // size]
+        if used.numel() and not 0 <= int(used.min()) <= int(used.max()) < k_pages.shape[0]:
+            raise IndexError(f"sequence {s}: a page outside [0, {k_pages.shape[0]})")
+        a, b = offs[s], offs[s + 1]
+        if offsets is None and n == 0:
+            b = a    # an idle slot
+        if not 0 <= a <= b <= rows or b - a > n:
+            raise IndexError(f"sequence {s}: rows {a}..{b} of {rows}, length {n}")
+        out.append((s, a, b - a, n))
+    return out
+
+
+def _append_cpu(x, k_pages, v_pages, table, lengths, offsets, n_heads, theta):
+    hkv, size, D = k_pages.shape[1:]
+    q = torch.zeros(x.shape[0], n_heads, D, dtype=x.dtype, device=x.device)
+    for s, at, n, total in _runs(k_pages, table, lengths, offsets, x.shape[0]):
+        pos = torch.arange(total - n, total)
+        rows = x[at:at + n]
+        if theta is not None:
+            angle = pos.double()[:, None] * theta ** (-2.0 * torch.arange(D // 2, dtype=torch.float64) / D)
+            f = torch.promote_types(x.dtype, torch.float32)
+            cs, sn = angle.cos().to(f)[:, None], angle.sin().to(f)[:, None]
+            a, b = rows[:, :n_heads + hkv, :D // 2].to(f), rows[:, :n_heads + hkv, D // 2:].to(f)
+            turned = torch.cat([a * cs - b * sn, b * cs + a * sn], -1).to(x.dtype)
+            rows = torch.cat([turned, rows[:, n_heads + hkv:]], 1)
+        q[at:at + n] = rows[:, :n_heads]
+        page, slot = table[s].long()[pos // size], pos % size
+        k_pages[page, :, slot] = rows[:, n_heads:n_heads + hkv]
+        v_pages[page, :, slot] = rows[:, n_heads + hkv:]
+    return q
+
+
+def _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale):
+    hkv, size, D = k_pages.shape[1:]
+    out = torch.zeros(q.shape, dtype=q.dtype)
+    f = torch.promote_types(q.dtype, torch.float32)
+    group = q.shape[1] // hkv
+    for s, at, n, total in _runs(k_pages, table, lengths, offsets, q.shape[0]):
+        pages = table[s, :(total + size - 1) // size].long()
+        k, v = (t[pages].transpose(0, 1).reshape(hkv, -1, D)[:, :total].to(f).repeat_interleave(group, 0) for t in (k_pages, v_pages))
+        z = torch.einsum("nhd,hkd->hnk", q[at:at + n].to(f), k) * scale
+        for i in range(n):   # row by row, so that a key behind a row's last one does not enter it, not even as 0 * NaN
+            seen = total - n + i + 1
+            out[at + i] = torch.einsum("hk,hkd->hd", torch.softmax(z[:, i, :seen], -1), v[:, :seen]).to(q.dtype)
+    return out

@@ -120,6 +120,39 @@ pub struct incin_attn_desc {
 
 #[repr(C)]
 #[derive(Clone, Copy)]
+pub struct incin_paged_desc {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub k_stride_page: c_longlong,
+    pub k_stride_head: c_longlong,
+    pub k_stride_token: c_longlong,
+    pub v_stride_page: c_longlong,
+    pub v_stride_head: c_longlong,
+    pub v_stride_token: c_longlong,
+    pub table: *const i32,
+    pub table_stride: c_longlong,
+    pub lengths: *const i32,
+    pub offsets: *const i32,
+    pub table_width: c_int,
+    pub seqs: c_int,
+    pub rows: c_int,
+    pub pages: c_int,
+    pub page_size: c_int,
+    pub Hq: c_int,
+    pub Hkv: c_int,
+    pub D: c_int,
+    pub dtype: c_int,
+    pub scale: f32,
+    pub x: *const c_void,
+    pub x_stride_row: c_longlong,
+    pub x_stride_head: c_longlong,
+    pub out: *mut c_void,
+    pub workspace: *mut c_void,
+    pub status: *mut c_void,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
 pub struct incin_conv_geom {
     pub N: c_int,
     pub C: c_int,
@@ -180,6 +213,7 @@ extern "C" {
     pub fn incin_colsum_scratch_floats(rows: c_longlong, N: c_int) -> c_longlong;
     pub fn incin_colsum_typed(dy: *const c_void, out: *mut c_void, scratch: *mut f32, rows: c_longlong, N: c_int, ld: c_longlong, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn incin_conv_out_hw(g: *const incin_conv_geom, oh: *mut c_int, ow: *mut c_int) -> c_int;
+    pub fn incin_copy_pages(storage: *mut c_void, src: *const i32, dst: *const i32, pairs: c_int, outer: c_longlong, pages: c_int, page_bytes: c_longlong, status: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn incin_cpu_adamw_f32(w: *mut f32, m: *mut f32, v: *mut f32, g: *const f32, n: i64, lr: f32, b1: f32, b2: f32, eps: f32, wd: f32, step: c_int);
     pub fn incin_cpu_attention_f32(q: *const f32, k: *const f32, v: *const f32, o: *mut f32, heads: i64, T: i64, D: i64, scale: f32, causal: c_int);
     pub fn incin_cpu_cross_entropy_f32(logits: *const f32, targets: *const i64, dlogits: *mut f32, rows: i64, V: i64) -> f32;
@@ -195,6 +229,8 @@ extern "C" {
     pub fn incin_cpu_softmax_f32(x: *const f32, y: *mut f32, rows: i64, C: i64, log_softmax: c_int);
     pub fn incin_cpu_unary_f32(x: *const f32, y: *mut f32, n: i64, op: c_int);
     pub fn incin_cumsum(x: *const c_void, out: *mut c_void, outer: c_longlong, n: c_longlong, inner: c_longlong, is_bf16: c_int, stream: *mut c_void) -> c_int;
+    pub fn incin_decode_attention(desc: *const incin_paged_desc, stream: *mut c_void) -> c_int;
+    pub fn incin_decode_attention_workspace(desc: *const incin_paged_desc) -> c_longlong;
     pub fn incin_dequantize_q8_0(packed: *const c_void, out: *mut c_void, n: c_longlong, out_bf16: c_int, stream: *mut c_void) -> c_int;
     pub fn incin_digest_bytes(state: u64, data: *const c_void, n: i64) -> u64;
     pub fn incin_digest_field(state: u64, data: *const c_void, n: i64) -> u64;
@@ -216,6 +252,7 @@ extern "C" {
     pub fn incin_gather_rows(src: *const c_void, index: *const c_longlong, out: *mut c_void, n_idx: c_longlong, row_elems: c_longlong, src_rows: c_longlong, elem_bytes: c_int, err_flag: *mut c_int, stream: *mut c_void) -> c_int;
     pub fn incin_gemm_bf16(desc: *const incin_gemm_desc, stream: *mut c_void) -> c_int;
     pub fn incin_im2col(x: *const c_void, cols: *mut c_void, g: *const incin_conv_geom, is_bf16: c_int, stream: *mut c_void) -> c_int;
+    pub fn incin_kv_append(desc: *const incin_paged_desc, theta: f64, stream: *mut c_void) -> c_int;
     pub fn incin_layernorm_bwd(dy: *const c_void, x: *const c_void, gamma: *const c_void, mean: *const f32, rstd: *const f32, dx_add: *const c_void, dx: *mut c_void, dgamma: *mut f32, dbeta: *mut f32, scratch: *mut f32, rows: c_longlong, C: c_int, stream: *mut c_void) -> c_int;
     pub fn incin_layernorm_bwd_colsum(dy: *const c_void, x: *const c_void, gamma: *const c_void, mean: *const f32, rstd: *const f32, dx_add: *const c_void, dx: *mut c_void, dgamma: *mut f32, dbeta: *mut f32, dxsum: *mut f32, scratch: *mut f32, rows: c_longlong, C: c_int, stream: *mut c_void) -> c_int;
     pub fn incin_layernorm_bwd_colsum_scratch_floats(rows: c_longlong, C: c_int) -> c_longlong;
@@ -239,6 +276,8 @@ extern "C" {
     pub fn incin_philox_normal_bf16(out: *mut c_void, n: c_longlong, seed: u64, offset: u64, mean: f32, std: f32, stream: *mut c_void) -> c_int;
     pub fn incin_philox_normal_f32(out: *mut f32, n: c_longlong, seed: u64, offset: u64, mean: f32, std: f32, stream: *mut c_void) -> c_int;
     pub fn incin_philox_uniform_f32(out: *mut f32, n: c_longlong, seed: u64, offset: u64, stream: *mut c_void) -> c_int;
+    pub fn incin_prompt_attention(desc: *const incin_paged_desc, stream: *mut c_void) -> c_int;
+    pub fn incin_prompt_attention_workspace(desc: *const incin_paged_desc) -> c_longlong;
     pub fn incin_quantize_q8_0(x: *const c_void, packed: *mut c_void, n: c_longlong, is_bf16: c_int, stream: *mut c_void) -> c_int;
     pub fn incin_rdv_abort(h: i64, code: c_int, timeout_ms: c_int) -> c_int;
     pub fn incin_rdv_allgather(h: i64, mine: *const c_void, bytes: c_int, all: *mut c_void, timeout_ms: c_int) -> c_int;
