@@ -92,13 +92,6 @@ static int attend(const incin_paged_desc* d, void* stream) {
 
 }  // namespace incin
 
-extern "C" long long incin_decode_attention_workspace(const incin_paged_desc*) { return 0; }
-extern "C" int incin_decode_attention(const incin_paged_desc* d, void* stream) {
-  if (!d || d->rows != d->seqs) return INCIN_ERR_ARGUMENT;
-  incin_paged_desc one = *d;
-  one.offsets = nullptr;
-  return incin::attend(&one, stream);
-}
 extern "C" long long incin_prompt_attention_workspace(const incin_paged_desc*) { return 0; }
 extern "C" int incin_prompt_attention(const incin_paged_desc* d, void* stream) {
   if (!d || !d->offsets) return INCIN_ERR_ARGUMENT;

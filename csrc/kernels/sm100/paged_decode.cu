@@ -1,0 +1,460 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   o_h = sum_j p_hj v_j,  p_hj = 2^(z_hj - m_h) / l_h,  z = scale log2(e) q_h k_j,  j < lengths[b]
+//
+// Every cached key and value is used once, so the bytes of the cache bound it.  The query heads of a key head are the
+// columns of one product: S^T [16 keys x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T with m16n8k16 matrix
+// instructions (tcgen05.mma wants 128 rows; here a row of its operand would be a key that is used for 8 columns, and the
+// tiles would have to pass through shared memory).  Both operands go from global memory straight into the registers that the instructions read,
+// 16 bytes a load: the order in which a product runs over D, and in which its rows of V^T are numbered, is free, so it is
+// chosen to be the order in which the bytes arrive.  K: lane (r, c) = (lane / 4, lane % 4) loads key rows r and r + 8 at
+// element 32 j + 8 c: its four 32-bit words are the k indices of two instructions, and the queries are held in the same order.
+// V: it loads keys 2c, 2c + 1, 2c + 8, 2c + 9 at element 64 j + 8 r; a pair of keys and a word make two rows of V^T by two
+// byte permutes.  P^T comes out of S^T by transposing 8 x 8 blocks between the lanes (movmatrix).  No shared memory, no
+// barrier in the loop: a warp asks for its next keys as soon as the present ones are used, and values likewise.
+//
+// Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal
+// run of all units, each warp every fourth 16 keys of it.  A pair of sequence and head that crosses CTAs leaves fp32 parts
+// (O, m, l), which a second kernel joins in a fixed order.  So the lengths are needed on the device only, one long
+// sequence uses all SMs, and a captured launch stays balanced whatever its lengths become.
+#include "paged.cuh"
+
+#include <math_constants.h>
+
+namespace incin {
+
+constexpr int DEC_WARPS = 4, DEC_UNIT = 16 * DEC_WARPS;
+constexpr int DEC_SEQS = 1024;   // sequences a launch
+
+template <int D, int NT>
+struct DecCfg {   // NT: blocks of 8 query heads
+  static constexpr int HEADS = 8 * NT;
+  static constexpr int CTAS_PER_SM = NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);
+  static constexpr int SLOT = HEADS * (D + 2);   // floats of a part: O [HEADS][D], m [HEADS], l [HEADS]
+  static constexpr int ROW = D + 4;              // of O in shared memory
+};
+
+struct DecParams {
+  PagedView c;
+  const uint16_t* x;
+  long long x_row, x_head;
+  uint16_t* out;
+  float scale_log2;
+  int group, chunks;   // query heads of a key head, and the blocks of HEADS they are dealt in
+  int4* open;          // per CTA: {sequence, head block, last CTA} of the pair that it begins and others continue, or -1
+  float* parts;        // per CTA two slots: the continuation of a pair, the beginning of one
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<Bf16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<Fp16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transpose of an 8 x 8 block of 16-bit elements held in the accumulator's order
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// 16 bytes that no other load wants again; zeros where `there` is false (nothing is read then)
+__device__ __forceinline__ void load16(uint32_t (&w)[4], const uint16_t* p, bool there) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0;\n"
+      "@p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+      "}\n"
+      : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
+      : "l"(p), "r"((int)there));
+}
+
+// First unit of CTA i of n over `units` units
+__device__ __forceinline__ long long dec_start(long long units, int i, int n) { return units * i / n; }
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) decode_attention_kernel(const DecParams p) {
+  using Cfg = DecCfg<D, NT>;
+  constexpr int KJ = D / 32, VJ = D / 64;
+  __shared__ long long before[DEC_SEQS + 1];   // units of one head in front of each sequence
+  __shared__ int length[DEC_SEQS];
+  __shared__ long long warp_sum[DEC_WARPS];
+  __shared__ float sm_m[DEC_WARPS][Cfg::HEADS], sm_l[DEC_WARPS][Cfg::HEADS];
+  __shared__ __align__(16) float sm_o[DEC_WARPS][Cfg::HEADS][Cfg::ROW];
+  const PagedView& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q4 = lane & 3;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  {   // units in front of each sequence; one without tokens has a unit too, which writes its zeros
+    const int per = (c.seqs + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32), s0 = threadIdx.x * per;
+    long long sum = 0;
+    for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
+      length[s] = paged_length(c, s);
+      sum += max(1, (length[s] + DEC_UNIT - 1) / DEC_UNIT);
+    }
+    long long incl = sum;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, incl, w);
+      if (lane >= w) incl += other;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    long long at = incl - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sum[w];
+    for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
+      before[s] = at;
+      at += max(1, (length[s] + DEC_UNIT - 1) / DEC_UNIT);
+      if (s == c.seqs - 1) before[c.seqs] = at;
+    }
+    __syncthreads();
+  }
+  const int head_blocks = c.Hkv * p.chunks;
+  const long long units = before[c.seqs] * head_blocks;
+  const int ctas = (int)min((long long)gridDim.x, units);
+  if ((int)blockIdx.x >= ctas) {
+    if (threadIdx.x == 0) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+  long long u = dec_start(units, blockIdx.x, ctas);
+  const long long u_end = dec_start(units, blockIdx.x + 1, ctas);
+  int4 opened = make_int4(-1, 0, 0, 0);
+  int b;
+  {
+    int lo = 0, hi = c.seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (before[mid] * head_blocks <= u) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+  }
+  while (u < u_end) {
+    while (before[b + 1] * head_blocks <= u) ++b;
+    const int n_units = (int)(before[b + 1] - before[b]);
+    const long long rest = u - before[b] * head_blocks;
+    const int hb = (int)(rest / n_units), t0 = (int)(rest % n_units);
+    const int t1 = (int)min((long long)n_units, t0 + (u_end - u));
+    const int hk = hb / p.chunks, h0 = hb % p.chunks * Cfg::HEADS, heads = min(Cfg::HEADS, p.group - h0);
+    const int key_end = min(length[b], t1 * DEC_UNIT);
+    const uint16_t* kb = c.k + hk * c.k_head;
+    const uint16_t* vb = c.v + hk * c.v_head;
+
+    uint32_t q[NT][KJ][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+        load16(q[t][j], p.x + b * p.x_row + (hk * p.group + h0 + t * 8 + r) * p.x_head + j * 32 + q4 * 8, t * 8 + r < heads);
+    float o[NT][VJ][4][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -CUDART_INF_F;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < VJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][j][i][e] = 0.f;
+    }
+
+    // 16 keys from `key` on: one page, since pages begin at multiples of 16.  A lane holds the pages of one of the next 32 steps.
+    const int first = (t0 * DEC_WARPS + warp) * 16;
+    int pages = -1;
+    auto fetch_pages = [&](int key) {
+      const int mine = key + lane * DEC_UNIT;
+      pages = mine < key_end ? paged_page(c, b, mine >> c.page_shift) : -1;
+    };
+    uint32_t kr[2][KJ][4], vr[4][VJ][4];
+    auto load_k = [&](int key, int page) {
+      const uint16_t* base = kb + page * c.k_page + (key & ((1 << c.page_shift) - 1)) * c.k_token;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool there = page >= 0 && key + r + i * 8 < key_end;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) load16(kr[i][j], base + (r + i * 8) * c.k_token + j * 32 + q4 * 8, there);
+      }
+    };
+    auto load_v = [&](int key, int page) {
+      const uint16_t* base = vb + page * c.v_page + (key & ((1 << c.page_shift) - 1)) * c.v_token;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = q4 * 2 + (i & 1) + (i >> 1) * 8;
+        const bool there = page >= 0 && key + row < key_end;
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + row * c.v_token + j * 64 + r * 8, there);
+      }
+    };
+    int step = 0;
+    fetch_pages(first);
+    if (first < key_end) {
+      const int page = __shfl_sync(0xffffffffu, pages, 0);
+      load_k(first, page);
+      load_v(first, page);
+    }
+    for (int key = first; key < key_end; key += DEC_UNIT) {
+      const int next = key + DEC_UNIT;
+      if ((++step & 31) == 0) fetch_pages(next);
+      const int next_page = __shfl_sync(0xffffffffu, pages, step & 31);
+      float s[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          mma16816<T>(even, kr[0][j][0], kr[1][j][0], kr[0][j][1], kr[1][j][1], q[t][j][0], q[t][j][1]);
+          mma16816<T>(odd, kr[0][j][2], kr[1][j][2], kr[0][j][3], kr[1][j][3], q[t][j][2], q[t][j][3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = (even[e] + odd[e]) * p.scale_log2;
+      }
+      if (next < key_end) load_k(next, next_page);
+      if (key + 16 > key_end) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key + r + (e >> 1) * 8 >= key_end) s[t][e] = -CUDART_INF_F;
+      }
+      // element e of s: key r (+ 8 from e = 2 on), head 2 q4 + (e & 1).  The reference of the exponentials moves only when
+      // the maximum has grown by more than 2^8; O and l are divided by each other in the end.
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float mx[2] = {fmaxf(s[t][0], s[t][2]), fmaxf(s[t][1], s[t][3])};
+        if (__any_sync(0xffffffffu, mx[0] > m[t][0] + 8.f || mx[1] > m[t][1] + 8.f)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
+            const bool move = mx[e] > m[t][e] + 8.f;
+            const float alpha = move ? exp2f(m[t][e] - mx[e]) : 1.f;
+            if (move) m[t][e] = mx[e];
+            l[t][e] *= alpha;
+#pragma unroll
+            for (int j = 0; j < VJ; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                o[t][j][i][e] *= alpha;
+                o[t][j][i][e + 2] *= alpha;
+              }
+          }
+        }
+        const float r0 = m[t][0] == -CUDART_INF_F ? 0.f : m[t][0], r1 = m[t][1] == -CUDART_INF_F ? 0.f : m[t][1];
+        const float p0 = exp2f(s[t][0] - r0), p1 = exp2f(s[t][1] - r1), p2 = exp2f(s[t][2] - r0), p3 = exp2f(s[t][3] - r1);
+        l[t][0] += p0 + p2;
+        l[t][1] += p1 + p3;
+        // P in the cache's type, as the instruction wants it: half a step of relative error a weight
+        pb[t][0] = transpose8x8(T::pack(p0, p1));
+        pb[t][1] = transpose8x8(T::pack(p2, p3));
+      }
+#pragma unroll
+      for (int j = 0; j < VJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // rows 64 j + 8 r + 2 i and + 1 of V^T
+          const uint32_t a0 = __byte_perm(vr[0][j][i], vr[1][j][i], 0x5410), a1 = __byte_perm(vr[0][j][i], vr[1][j][i], 0x7632);
+          const uint32_t a2 = __byte_perm(vr[2][j][i], vr[3][j][i], 0x5410), a3 = __byte_perm(vr[2][j][i], vr[3][j][i], 0x7632);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816<T>(o[t][j][i], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+        }
+      if (next < key_end) load_v(next, next_page);
+    }
+
+    // join the warps
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], w);
+        if (r == 0) {
+          sm_m[warp][t * 8 + q4 * 2 + e] = m[t][e];
+          sm_l[warp][t * 8 + q4 * 2 + e] = l[t][e];
+        }
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) {
+          float4* row = reinterpret_cast<float4*>(&sm_o[warp][t * 8 + q4 * 2 + e][j * 64 + r * 8]);
+          row[0] = make_float4(o[t][j][0][e], o[t][j][0][e + 2], o[t][j][1][e], o[t][j][1][e + 2]);
+          row[1] = make_float4(o[t][j][2][e], o[t][j][2][e + 2], o[t][j][3][e], o[t][j][3][e + 2]);
+        }
+      }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == n_units;
+    float* slot = p.parts + (2ll * blockIdx.x + (t0 == 0)) * Cfg::SLOT;
+    for (int i = threadIdx.x; i < Cfg::HEADS * (D / 8); i += DEC_WARPS * 32) {
+      const int h = i / (D / 8), d = i % (D / 8) * 8;
+      if (h >= heads) continue;
+      float top = -CUDART_INF_F, sum = 0.f, acc[8] = {};
+#pragma unroll
+      for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, sm_m[w][h]);
+#pragma unroll
+      for (int w = 0; w < DEC_WARPS; ++w) {
+        // a warp without keys has m = -inf, l = 0 and O = 0
+        const float f = sm_m[w][h] == top ? 1.f : exp2f(sm_m[w][h] - top);
+        sum += f * sm_l[w][h];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += f * sm_o[w][h][d + e];
+      }
+      if (whole) {
+        const float inv = key_end > 0 ? 1.f / sum : 0.f;
+        *reinterpret_cast<uint4*>(p.out + ((long long)b * c.Hq + hk * p.group + h0 + h) * D + d) =
+            make_uint4(T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv), T::pack(acc[4] * inv, acc[5] * inv),
+                       T::pack(acc[6] * inv, acc[7] * inv));
+      } else {
+        float4* dst = reinterpret_cast<float4*>(slot + h * D + d);
+        dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        if (d == 0) {
+          slot[Cfg::HEADS * D + h] = top;
+          slot[Cfg::HEADS * (D + 1) + h] = sum;
+        }
+      }
+    }
+    if (t0 == 0 && !whole) {
+      const long long last_unit = before[b] * head_blocks + (long long)(hb + 1) * n_units - 1;
+      opened = make_int4(b, hb, (int)(((last_unit + 1) * ctas - 1) / units), 0);
+    }
+    __syncthreads();
+    u += t1 - t0;
+  }
+  if (threadIdx.x == 0) p.open[blockIdx.x] = opened;
+}
+
+// Block (i, h): joins the parts of the pair that CTA i began, if it began one, for one query head.
+constexpr int JOIN_THREADS = 256;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(JOIN_THREADS) decode_join_kernel(const DecParams p) {
+  using Cfg = DecCfg<D, NT>;
+  constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / LANES;
+  extern __shared__ float weight[];   // a part each
+  __shared__ float4 acc_of[GROUPS][LANES];
+  __shared__ float red[2][JOIN_THREADS / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int4 pair = p.open[blockIdx.x];
+  const int h = blockIdx.y, h0 = pair.y % p.chunks * Cfg::HEADS, hk = pair.y / p.chunks;
+  if (pair.x < 0 || h >= p.group - h0) return;
+  const int begin = blockIdx.x, parts = pair.z - begin + 1;
+  auto slot = [&](int i) { return p.parts + (2ll * (begin + i) + (i == 0)) * Cfg::SLOT; };
+  float top = -CUDART_INF_F;
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
+    weight[i] = slot(i)[Cfg::HEADS * D + h];
+    top = fmaxf(top, weight[i]);
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, red[0][w]);
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
+    const float f = weight[i] == top ? 1.f : exp2f(weight[i] - top);
+    weight[i] = f;
+    sum += f * slot(i)[Cfg::HEADS * (D + 1) + h];
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  if ((threadIdx.x & 31) == 0) red[1][threadIdx.x >> 5] = sum;
+  __syncthreads();
+  const int lane = threadIdx.x % LANES, g = threadIdx.x / LANES;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = g; i < parts; i += GROUPS) {
+    const float f = weight[i];
+    const float4 v = reinterpret_cast<const float4*>(slot(i) + h * D)[lane];
+    acc = make_float4(acc.x + f * v.x, acc.y + f * v.y, acc.z + f * v.z, acc.w + f * v.w);
+  }
+  acc_of[g][lane] = acc;
+  __syncthreads();
+  if (g) return;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += red[1][w];
+#pragma unroll
+  for (int w = 1; w < GROUPS; ++w) {
+    const float4 v = acc_of[w][lane];
+    acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+  }
+  const float inv = 1.f / sum;
+  *reinterpret_cast<uint2*>(p.out + ((long long)pair.x * p.c.Hq + hk * p.group + h0 + h) * D + lane * 4) =
+      make_uint2(T::pack(acc.x * inv, acc.y * inv), T::pack(acc.z * inv, acc.w * inv));
+}
+
+struct DecPlan {
+  int grid, chunks;
+  bool splits;   // whether a pair can cross CTAs
+  long long bytes;
+};
+
+template <int D, int NT>
+static DecPlan dec_plan(const incin_paged_desc* d) {
+  using Cfg = DecCfg<D, NT>;
+  DecPlan pl;
+  pl.chunks = (d->Hq / d->Hkv + Cfg::HEADS - 1) / Cfg::HEADS;
+  const long long seqs = d->seqs < DEC_SEQS ? d->seqs : DEC_SEQS;
+  const long long per_pair = ((long long)d->table_width * d->page_size + DEC_UNIT - 1) / DEC_UNIT;
+  const long long most = seqs * d->Hkv * pl.chunks * per_pair;
+  const long long room = (long long)device_sm_count() * Cfg::CTAS_PER_SM;
+  pl.grid = (int)(most < room ? most : room);
+  pl.splits = per_pair > 1;
+  pl.bytes = (long long)pl.grid * (16 + 2 * Cfg::SLOT * 4);
+  return pl;
+}
+
+template <typename T, int D, int NT>
+static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
+  using Cfg = DecCfg<D, NT>;
+  const DecPlan pl = dec_plan<D, NT>(d);
+  DecParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
+                 d->Hq / d->Hkv, pl.chunks, (int4*)d->workspace, (float*)((char*)d->workspace + 16ll * pl.grid)};
+  p.c.offsets = nullptr;
+  for (int s0 = 0; s0 < d->seqs; s0 += DEC_SEQS) {
+    DecParams q = p;
+    q.c.seqs = q.c.rows = d->seqs - s0 < DEC_SEQS ? d->seqs - s0 : DEC_SEQS;
+    q.c.table += s0 * d->table_stride;
+    q.c.lengths += s0;
+    q.x += s0 * d->x_stride_row;
+    q.out += (long long)s0 * d->Hq * D;
+    if (launch_pdl<true>(decode_attention_kernel<T, D, NT>, dim3(pl.grid), dim3(DEC_WARPS * 32), 0, stream, q) != cudaSuccess)
+      return INCIN_ERR_LAUNCH;
+    if (pl.splits && launch_pdl<true>(decode_join_kernel<T, D, NT>, dim3(pl.grid, Cfg::HEADS), dim3(JOIN_THREADS), pl.grid * sizeof(float), stream,
+                                      q) != cudaSuccess)
+      return INCIN_ERR_LAUNCH;
+  }
+  return INCIN_OK;
+}
+
+}  // namespace incin
+
+extern "C" long long incin_decode_attention_workspace(const incin_paged_desc* d) {
+  using namespace incin;
+  if (!d || d->Hkv <= 0 || d->Hq <= 0) return 0;
+  const bool one = d->Hq / d->Hkv <= 8;
+  if (d->D == 64) return one ? dec_plan<64, 1>(d).bytes : dec_plan<64, 2>(d).bytes;
+  return one ? dec_plan<128, 1>(d).bytes : dec_plan<128, 2>(d).bytes;
+}
+
+extern "C" int incin_decode_attention(const incin_paged_desc* d, void* stream) {
+  using namespace incin;
+  const int rc = check_paged(d);
+  if (rc) return rc;
+  if (d->rows != d->seqs || !d->workspace) return INCIN_ERR_ARGUMENT;
+  const cudaStream_t s = (cudaStream_t)stream;
+  const bool one = d->Hq / d->Hkv <= 8;
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    if (d->D == 64) return one ? launch_decode<T, 64, 1>(d, s) : launch_decode<T, 64, 2>(d, s);
+    return one ? launch_decode<T, 128, 1>(d, s) : launch_decode<T, 128, 2>(d, s);
+  };
+  return d->dtype == INCIN_GEMM_IN_FP16 ? run(Fp16()) : run(Bf16());
+}
