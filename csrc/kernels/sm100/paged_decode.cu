@@ -13,8 +13,8 @@
 // byte permutes.  P^T comes out of S^T by transposing 8 x 8 blocks between the lanes (movmatrix).  No shared memory, no
 // barrier in the loop: a warp asks for its next keys as soon as the present ones are used, and values likewise.
 //
-// Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal
-// run of all units, each warp every fourth 16 keys of it.  A pair of sequence and head that crosses CTAs leaves fp32 parts
+// Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal run of all
+// units, each warp 16 tokens of every one.  A pair of sequence and head that crosses CTAs leaves fp32 parts
 // (O, m, l), which a second kernel joins in a fixed order.  So the lengths are needed on the device only, one long
 // sequence uses all SMs, and a captured launch stays balanced whatever its lengths become.
 #include "paged.cuh"
@@ -23,15 +23,17 @@
 
 namespace incin {
 
-constexpr int DEC_WARPS = 4, DEC_UNIT = 16 * DEC_WARPS;
-constexpr int DEC_SEQS = 1024;   // sequences a launch
+constexpr int DEC_WARPS = 4, DEC_STEP = 16 * DEC_WARPS;   // keys a CTA takes at a time, 16 a warp
+constexpr int DEC_SEQS = 512;   // sequences a launch
 
 template <int D, int NT>
 struct DecCfg {   // NT: blocks of 8 query heads
   static constexpr int HEADS = 8 * NT;
-  static constexpr int CTAS_PER_SM = NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);
+  static constexpr int CTAS_PER_SM = (D == 64 ? 4 : 3) - (NT - 1);
   static constexpr int SLOT = HEADS * (D + 2);   // floats of a part: O [HEADS][D], m [HEADS], l [HEADS]
   static constexpr int ROW = D + 4;              // of O in shared memory
+  // of an SM's CTAs: O, m and l of the warps, the sequences' lengths and units, 1 KB each for the system
+  static constexpr int SHARED = CTAS_PER_SM * (DEC_WARPS * HEADS * (ROW + 2) * 4 + 8 * DEC_SEQS + 64 + 1024);
 };
 
 struct DecParams {
@@ -40,6 +42,7 @@ struct DecParams {
   long long x_row, x_head;
   uint16_t* out;
   float scale_log2;
+  int unit;            // tokens of a unit of work, a multiple of DEC_STEP
   int group, chunks;   // query heads of a key head, and the blocks of HEADS they are dealt in
   int4* open;          // per CTA: {sequence, head block, last CTA} of the pair that it begins and others continue, or -1
   float* parts;        // per CTA two slots: the continuation of a pair, the beginning of one
@@ -83,9 +86,9 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) decode_attention_kernel(const DecParams p) {
   using Cfg = DecCfg<D, NT>;
   constexpr int KJ = D / 32, VJ = D / 64;
-  __shared__ long long before[DEC_SEQS + 1];   // units of one head in front of each sequence
+  __shared__ int before[DEC_SEQS + 1];   // units of one head in front of each sequence
   __shared__ int length[DEC_SEQS];
-  __shared__ long long warp_sum[DEC_WARPS];
+  __shared__ int warp_sum[DEC_WARPS];
   __shared__ float sm_m[DEC_WARPS][Cfg::HEADS], sm_l[DEC_WARPS][Cfg::HEADS];
   __shared__ __align__(16) float sm_o[DEC_WARPS][Cfg::HEADS][Cfg::ROW];
   const PagedView& c = p.c;
@@ -95,30 +98,30 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
 
   {   // units in front of each sequence; one without tokens has a unit too, which writes its zeros
     const int per = (c.seqs + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32), s0 = threadIdx.x * per;
-    long long sum = 0;
+    int sum = 0;
     for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
       length[s] = paged_length(c, s);
-      sum += max(1, (length[s] + DEC_UNIT - 1) / DEC_UNIT);
+      sum += max(1, (length[s] + p.unit - 1) / p.unit);
     }
-    long long incl = sum;
+    int incl = sum;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, incl, w);
+      const int other = __shfl_up_sync(0xffffffffu, incl, w);
       if (lane >= w) incl += other;
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    long long at = incl - sum;
+    int at = incl - sum;
     for (int w = 0; w < warp; ++w) at += warp_sum[w];
     for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
       before[s] = at;
-      at += max(1, (length[s] + DEC_UNIT - 1) / DEC_UNIT);
+      at += max(1, (length[s] + p.unit - 1) / p.unit);
       if (s == c.seqs - 1) before[c.seqs] = at;
     }
     __syncthreads();
   }
   const int head_blocks = c.Hkv * p.chunks;
-  const long long units = before[c.seqs] * head_blocks;
+  const long long units = (long long)before[c.seqs] * head_blocks;
   const int ctas = (int)min((long long)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) {
     if (threadIdx.x == 0) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -127,32 +130,82 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   long long u = dec_start(units, blockIdx.x, ctas);
   const long long u_end = dec_start(units, blockIdx.x + 1, ctas);
   int4 opened = make_int4(-1, 0, 0, 0);
-  int b;
+  int b;   // the sequence of unit u
   {
     int lo = 0, hi = c.seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (before[mid] * head_blocks <= u) lo = mid; else hi = mid - 1;
+      if ((long long)before[mid] * head_blocks <= u) lo = mid; else hi = mid - 1;
     }
     b = lo;
   }
-  while (u < u_end) {
-    while (before[b + 1] * head_blocks <= u) ++b;
-    const int n_units = (int)(before[b + 1] - before[b]);
-    const long long rest = u - before[b] * head_blocks;
-    const int hb = (int)(rest / n_units), t0 = (int)(rest % n_units);
-    const int t1 = (int)min((long long)n_units, t0 + (u_end - u));
-    const int hk = hb / p.chunks, h0 = hb % p.chunks * Cfg::HEADS, heads = min(Cfg::HEADS, p.group - h0);
-    const int key_end = min(length[b], t1 * DEC_UNIT);
-    const uint16_t* kb = c.k + hk * c.k_head;
-    const uint16_t* vb = c.v + hk * c.v_head;
 
-    uint32_t q[NT][KJ][4];
+  // A run of units of one pair of sequence and key head.
+  int n_units, hb, t0, t1, key_end;
+  auto enter = [&](int& seq, long long unit) {
+    while ((long long)before[seq + 1] * head_blocks <= unit) ++seq;
+    n_units = before[seq + 1] - before[seq];
+    const long long rest = unit - (long long)before[seq] * head_blocks;
+    hb = (rest >> 32) ? (int)(rest / n_units) : (int)((uint32_t)rest / (uint32_t)n_units);
+    t0 = (int)(rest - (long long)hb * n_units);
+    t1 = (int)min((long long)n_units, t0 + (u_end - unit));
+    key_end = (int)min((long long)length[seq], (long long)t1 * p.unit);
+  };
+  // 16 keys from a multiple of 16 on lie in one page.  A lane holds the page of one of the next 32 steps of its warp.
+  auto pages_from = [&](int seq, int key) {
+    const int mine = key + lane * DEC_STEP;
+    return mine < key_end ? paged_page(c, seq, mine >> c.page_shift) : -1;
+  };
+  uint32_t q[NT][KJ][4], kr[2][KJ][4], vr[4][VJ][4];
+  auto load_q = [&]() {
+    const int first_head = hb / p.chunks * p.group + hb % p.chunks * Cfg::HEADS, heads = p.group - hb % p.chunks * Cfg::HEADS;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
-        load16(q[t][j], p.x + b * p.x_row + (hk * p.group + h0 + t * 8 + r) * p.x_head + j * 32 + q4 * 8, t * 8 + r < heads);
+        load16(q[t][j], p.x + b * p.x_row + (first_head + t * 8 + r) * p.x_head + j * 32 + q4 * 8, t * 8 + r < heads);
+  };
+  int pages;   // -1 where there is none
+  auto load_k = [&](int key, int step) {
+    const uint16_t* kb = c.k + hb / p.chunks * c.k_head;
+    const int page = __shfl_sync(0xffffffffu, pages, step);
+    const uint16_t* base = kb + page * c.k_page + (key & ((1 << c.page_shift) - 1)) * c.k_token;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool there = page >= 0 && key + r + i * 8 < key_end;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) load16(kr[i][j], base + (r + i * 8) * c.k_token + j * 32 + q4 * 8, there);
+    }
+  };
+  auto load_v = [&](int key, int step) {
+    const uint16_t* vb = c.v + hb / p.chunks * c.v_head;
+    const int page = __shfl_sync(0xffffffffu, pages, step);
+    const uint16_t* base = vb + page * c.v_page + (key & ((1 << c.page_shift) - 1)) * c.v_token;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = q4 * 2 + (i & 1) + (i >> 1) * 8;
+      const bool there = page >= 0 && key + row < key_end;
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + row * c.v_token + j * 64 + r * 8, there);
+    }
+  };
+  enter(b, u);
+  pages = pages_from(b, t0 * p.unit + warp * 16);
+  load_q();
+  load_k(t0 * p.unit + warp * 16, 0);
+  load_v(t0 * p.unit + warp * 16, 0);
+
+  while (true) {
+    const int first = t0 * p.unit + warp * 16;
+    const long long next_u = u + (t1 - t0);
+    int next_pages = -1;
+    if (next_u < u_end) {   // asked for now, needed when this run ends
+      const int keep[5] = {n_units, hb, t0, t1, key_end};
+      int next_b = b;
+      enter(next_b, next_u);
+      next_pages = pages_from(next_b, t0 * p.unit + warp * 16);
+      n_units = keep[0], hb = keep[1], t0 = keep[2], t1 = keep[3], key_end = keep[4];
+    }
     float o[NT][VJ][4][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -167,44 +220,13 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           for (int e = 0; e < 4; ++e) o[t][j][i][e] = 0.f;
     }
 
-    // 16 keys from `key` on: one page, since pages begin at multiples of 16.  A lane holds the pages of one of the next 32 steps.
-    const int first = (t0 * DEC_WARPS + warp) * 16;
-    int pages = -1;
-    auto fetch_pages = [&](int key) {
-      const int mine = key + lane * DEC_UNIT;
-      pages = mine < key_end ? paged_page(c, b, mine >> c.page_shift) : -1;
-    };
-    uint32_t kr[2][KJ][4], vr[4][VJ][4];
-    auto load_k = [&](int key, int page) {
-      const uint16_t* base = kb + page * c.k_page + (key & ((1 << c.page_shift) - 1)) * c.k_token;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool there = page >= 0 && key + r + i * 8 < key_end;
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) load16(kr[i][j], base + (r + i * 8) * c.k_token + j * 32 + q4 * 8, there);
+    int step = 0;   // of the steps whose pages the lanes hold
+    for (int key = first; key < key_end; key += DEC_STEP) {
+      const int next = key + DEC_STEP;
+      if (++step == 32) {
+        step = 0;
+        pages = pages_from(b, next);
       }
-    };
-    auto load_v = [&](int key, int page) {
-      const uint16_t* base = vb + page * c.v_page + (key & ((1 << c.page_shift) - 1)) * c.v_token;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = q4 * 2 + (i & 1) + (i >> 1) * 8;
-        const bool there = page >= 0 && key + row < key_end;
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + row * c.v_token + j * 64 + r * 8, there);
-      }
-    };
-    int step = 0;
-    fetch_pages(first);
-    if (first < key_end) {
-      const int page = __shfl_sync(0xffffffffu, pages, 0);
-      load_k(first, page);
-      load_v(first, page);
-    }
-    for (int key = first; key < key_end; key += DEC_UNIT) {
-      const int next = key + DEC_UNIT;
-      if ((++step & 31) == 0) fetch_pages(next);
-      const int next_page = __shfl_sync(0xffffffffu, pages, step & 31);
       float s[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -217,7 +239,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[t][e] = (even[e] + odd[e]) * p.scale_log2;
       }
-      if (next < key_end) load_k(next, next_page);
+      if (next < key_end) load_k(next, step);
+      // element e of s: key r (+ 8 from e = 2 on), head 2 q4 + (e & 1)
       if (key + 16 > key_end) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -225,8 +248,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           for (int e = 0; e < 4; ++e)
             if (key + r + (e >> 1) * 8 >= key_end) s[t][e] = -CUDART_INF_F;
       }
-      // element e of s: key r (+ 8 from e = 2 on), head 2 q4 + (e & 1).  The reference of the exponentials moves only when
-      // the maximum has grown by more than 2^8; O and l are divided by each other in the end.
+      // The reference of the exponentials moves only when the maximum has grown by more than 2^8; O and l are divided by
+      // each other in the end.
       uint32_t pb[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -266,10 +289,19 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma16816<T>(o[t][j][i], a0, a1, a2, a3, pb[t][0], pb[t][1]);
         }
-      if (next < key_end) load_v(next, next_page);
+      if (next < key_end) load_v(next, step);
     }
 
-    // join the warps
+    // The keys, values and queries of the next run are on their way while the warps of this one are joined.
+    const int done_b = b, done_hb = hb, done_t0 = t0, done_t1 = t1, done_units = n_units, done_end = key_end;
+    u = next_u;
+    if (u < u_end) {
+      enter(b, u);
+      pages = next_pages;
+      load_q();
+      load_k(t0 * p.unit + warp * 16, 0);
+      load_v(t0 * p.unit + warp * 16, 0);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -288,8 +320,9 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         }
       }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == n_units;
-    float* slot = p.parts + (2ll * blockIdx.x + (t0 == 0)) * Cfg::SLOT;
+    const int h0 = done_hb % p.chunks * Cfg::HEADS, first_head = done_hb / p.chunks * p.group + h0, heads = min(Cfg::HEADS, p.group - h0);
+    const bool whole = done_t0 == 0 && done_t1 == done_units;
+    float* slot = p.parts + (2ll * blockIdx.x + (done_t0 == 0)) * Cfg::SLOT;
     for (int i = threadIdx.x; i < Cfg::HEADS * (D / 8); i += DEC_WARPS * 32) {
       const int h = i / (D / 8), d = i % (D / 8) * 8;
       if (h >= heads) continue;
@@ -305,8 +338,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         for (int e = 0; e < 8; ++e) acc[e] += f * sm_o[w][h][d + e];
       }
       if (whole) {
-        const float inv = key_end > 0 ? 1.f / sum : 0.f;
-        *reinterpret_cast<uint4*>(p.out + ((long long)b * c.Hq + hk * p.group + h0 + h) * D + d) =
+        const float inv = done_end > 0 ? 1.f / sum : 0.f;
+        *reinterpret_cast<uint4*>(p.out + ((long long)done_b * c.Hq + first_head + h) * D + d) =
             make_uint4(T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv), T::pack(acc[4] * inv, acc[5] * inv),
                        T::pack(acc[6] * inv, acc[7] * inv));
       } else {
@@ -319,79 +352,108 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         }
       }
     }
-    if (t0 == 0 && !whole) {
-      const long long last_unit = before[b] * head_blocks + (long long)(hb + 1) * n_units - 1;
-      opened = make_int4(b, hb, (int)(((last_unit + 1) * ctas - 1) / units), 0);
+    if (done_t0 == 0 && !whole) {
+      const long long last_unit = (long long)before[done_b] * head_blocks + (long long)(done_hb + 1) * done_units - 1;
+      opened = make_int4(done_b, done_hb, (int)(((last_unit + 1) * ctas - 1) / units), 0);
     }
+    if (u >= u_end) break;
     __syncthreads();
-    u += t1 - t0;
   }
   if (threadIdx.x == 0) p.open[blockIdx.x] = opened;
 }
 
-// Block (i, h): joins the parts of the pair that CTA i began, if it began one, for one query head.
+// Block (i, y): joins the parts of the pair that CTA i began, if it began one, for the query heads [y HB, (y + 1) HB).  A head
+// at a time (HB = 1) where the pairs are few, so that many parts each are read side by side.
 constexpr int JOIN_THREADS = 256;
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int HB>
 __global__ void __launch_bounds__(JOIN_THREADS) decode_join_kernel(const DecParams p) {
   using Cfg = DecCfg<D, NT>;
-  constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / LANES;
-  extern __shared__ float weight[];   // a part each
-  __shared__ float4 acc_of[GROUPS][LANES];
-  __shared__ float red[2][JOIN_THREADS / 32];
+  constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / (LANES * HB), PART_LANES = JOIN_THREADS / HB;   // threads of a head
+  constexpr int EARLY = 4;   // parts of O a thread asks for before it knows their weights
+  __shared__ float4 acc_of[HB][GROUPS][LANES];
+  __shared__ float red[HB][PART_LANES / 32], sum_of[HB][GROUPS];
   pdl_launch_dependents();
   pdl_wait();
   const int4 pair = p.open[blockIdx.x];
-  const int h = blockIdx.y, h0 = pair.y % p.chunks * Cfg::HEADS, hk = pair.y / p.chunks;
-  if (pair.x < 0 || h >= p.group - h0) return;
+  if (pair.x < 0) return;
+  const int mine = threadIdx.x / PART_LANES, tid = threadIdx.x % PART_LANES;
+  const int h = blockIdx.y * HB + mine, h0 = pair.y % p.chunks * Cfg::HEADS, hk = pair.y / p.chunks;
   const int begin = blockIdx.x, parts = pair.z - begin + 1;
   auto slot = [&](int i) { return p.parts + (2ll * (begin + i) + (i == 0)) * Cfg::SLOT; };
+  const int lane = tid % LANES, g = tid / LANES;
+  struct Part {
+    float4 o;
+    float m, l;
+  };
+  auto fetch = [&](int i) -> Part {
+    const float* at = slot(i);
+    return {reinterpret_cast<const float4*>(at + h * D)[lane], at[Cfg::HEADS * D + h], at[Cfg::HEADS * (D + 1) + h]};
+  };
+  Part early[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    if (g + i * GROUPS < parts) early[i] = fetch(g + i * GROUPS);
   float top = -CUDART_INF_F;
-  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
-    weight[i] = slot(i)[Cfg::HEADS * D + h];
-    top = fmaxf(top, weight[i]);
-  }
+  for (int i = tid; i < parts; i += PART_LANES) top = fmaxf(top, slot(i)[Cfg::HEADS * D + h]);
 #pragma unroll
   for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-  if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = top;
-  __syncthreads();
+  if (PART_LANES > 32) {
+    if ((tid & 31) == 0) red[mine][tid >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, red[0][w]);
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
-    const float f = weight[i] == top ? 1.f : exp2f(weight[i] - top);
-    weight[i] = f;
-    sum += f * slot(i)[Cfg::HEADS * (D + 1) + h];
+    for (int w = 0; w < PART_LANES / 32; ++w) top = fmaxf(top, red[mine][w]);
   }
-#pragma unroll
-  for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-  if ((threadIdx.x & 31) == 0) red[1][threadIdx.x >> 5] = sum;
-  __syncthreads();
-  const int lane = threadIdx.x % LANES, g = threadIdx.x / LANES;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  auto add = [&](const Part& a) {
+    const float f = a.m == top ? 1.f : exp2f(a.m - top);
+    sum += f * a.l;
+    acc = make_float4(acc.x + f * a.o.x, acc.y + f * a.o.y, acc.z + f * a.o.z, acc.w + f * a.o.w);
+  };
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    if (g + i * GROUPS < parts) add(early[i]);
 #pragma unroll 4
-  for (int i = g; i < parts; i += GROUPS) {
-    const float f = weight[i];
-    const float4 v = reinterpret_cast<const float4*>(slot(i) + h * D)[lane];
-    acc = make_float4(acc.x + f * v.x, acc.y + f * v.y, acc.z + f * v.z, acc.w + f * v.w);
-  }
-  acc_of[g][lane] = acc;
-  __syncthreads();
-  if (g) return;
-  sum = 0.f;
+  for (int i = g + EARLY * GROUPS; i < parts; i += GROUPS) add(fetch(i));
+  if (GROUPS > 1) {
+    acc_of[mine][g][lane] = acc;
+    if (lane == 0) sum_of[mine][g] = sum;
+    __syncthreads();
+    if (g) return;
 #pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += red[1][w];
-#pragma unroll
-  for (int w = 1; w < GROUPS; ++w) {
-    const float4 v = acc_of[w][lane];
-    acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+    for (int w = 1; w < GROUPS; ++w) {
+      const float4 v = acc_of[mine][w][lane];
+      acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+      sum += sum_of[mine][w];
+    }
   }
+  if (h >= p.group - h0) return;
   const float inv = 1.f / sum;
   *reinterpret_cast<uint2*>(p.out + ((long long)pair.x * p.c.Hq + hk * p.group + h0 + h) * D + lane * 4) =
       make_uint2(T::pack(acc.x * inv, acc.y * inv), T::pack(acc.z * inv, acc.w * inv));
 }
 
+// Loads in flight hold lines of the L1 cache, so the main kernel wants no more shared memory than its CTAs use, and the
+// joining kernel has to ask for the same split: a kernel that starts while another one runs keeps the split that it finds.
+// 256 sequences of up to 16384 tokens, 32 / 4 heads of 64: 339 us, 435 where the joining kernel took what it liked; with
+// the most shared memory 128 sequences of up to 8192, 24 / 8 heads of 128, take 467 in place of 332 us.
+template <typename Kern>
+static bool shared_split(Kern kern, int bytes, PerDeviceFlags& flags) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const bool tracked = dev >= 0 && dev < kMaxDevicesPerProcess;
+  if (tracked && __atomic_load_n(&flags.set[dev], __ATOMIC_ACQUIRE)) return true;
+  const int percent = (bytes * 100 + 228 * 1024 - 1) / (228 * 1024);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, percent) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (tracked) __atomic_store_n(&flags.set[dev], (unsigned char)1, __ATOMIC_RELEASE);
+  return true;
+}
+
 struct DecPlan {
-  int grid, chunks;
+  int grid, chunks, unit;
   bool splits;   // whether a pair can cross CTAs
   long long bytes;
 };
@@ -402,7 +464,13 @@ static DecPlan dec_plan(const incin_paged_desc* d) {
   DecPlan pl;
   pl.chunks = (d->Hq / d->Hkv + Cfg::HEADS - 1) / Cfg::HEADS;
   const long long seqs = d->seqs < DEC_SEQS ? d->seqs : DEC_SEQS;
-  const long long per_pair = ((long long)d->table_width * d->page_size + DEC_UNIT - 1) / DEC_UNIT;
+  const long long steps = ((long long)d->table_width * d->page_size + DEC_STEP - 1) / DEC_STEP;
+  // Where the table holds up to four steps, a pair stays with one CTA and the joining kernel is not needed: one sequence of 77
+  // tokens, 12 heads of 64, 6.0 -> 4.5 us.  (With eight steps the join is worth it: 8 sequences of up to 500, 32 / 4 heads of
+  // 64, 9.5 us a pair per CTA, 8.0 us split.)
+  const bool whole = steps <= 4;
+  pl.unit = DEC_STEP * (whole ? (int)steps : 1);
+  const long long per_pair = whole ? 1 : steps;
   const long long most = seqs * d->Hkv * pl.chunks * per_pair;
   const long long room = (long long)device_sm_count() * Cfg::CTAS_PER_SM;
   pl.grid = (int)(most < room ? most : room);
@@ -415,9 +483,14 @@ template <typename T, int D, int NT>
 static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
   using Cfg = DecCfg<D, NT>;
   const DecPlan pl = dec_plan<D, NT>(d);
+  if ((long long)d->table_width * d->page_size > (1ll << 37) / DEC_SEQS) return INCIN_ERR_TOO_LARGE;   // units are counted in 32 bits
   DecParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
-                 d->Hq / d->Hkv, pl.chunks, (int4*)d->workspace, (float*)((char*)d->workspace + 16ll * pl.grid)};
+                 pl.unit, d->Hq / d->Hkv, pl.chunks, (int4*)d->workspace, (float*)((char*)d->workspace + 16ll * pl.grid)};
   p.c.offsets = nullptr;
+  static PerDeviceFlags main_set, join_set, wide_join_set;
+  if (!shared_split(decode_attention_kernel<T, D, NT>, Cfg::SHARED, main_set) || !shared_split(decode_join_kernel<T, D, NT, 1>, Cfg::SHARED, join_set) ||
+      !shared_split(decode_join_kernel<T, D, NT, 8>, Cfg::SHARED, wide_join_set))
+    return INCIN_ERR_LAUNCH;
   for (int s0 = 0; s0 < d->seqs; s0 += DEC_SEQS) {
     DecParams q = p;
     q.c.seqs = q.c.rows = d->seqs - s0 < DEC_SEQS ? d->seqs - s0 : DEC_SEQS;
@@ -425,11 +498,15 @@ static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
     q.c.lengths += s0;
     q.x += s0 * d->x_stride_row;
     q.out += (long long)s0 * d->Hq * D;
-    if (launch_pdl<true>(decode_attention_kernel<T, D, NT>, dim3(pl.grid), dim3(DEC_WARPS * 32), 0, stream, q) != cudaSuccess)
-      return INCIN_ERR_LAUNCH;
-    if (pl.splits && launch_pdl<true>(decode_join_kernel<T, D, NT>, dim3(pl.grid, Cfg::HEADS), dim3(JOIN_THREADS), pl.grid * sizeof(float), stream,
-                                      q) != cudaSuccess)
-      return INCIN_ERR_LAUNCH;
+    // The main kernel is launched the ordinary way: 64 sequences of up to 4096, 32 / 4 heads of 64, 30.7 us, with programmatic
+    // launches of both kernels 36.9.
+    cudaError_t e = launch_pdl(decode_attention_kernel<T, D, NT>, dim3(pl.grid), dim3(DEC_WARPS * 32), 0, stream, q);
+    if (e != cudaSuccess) return INCIN_ERR_LAUNCH;
+    if (!pl.splits) continue;
+    const bool few = (long long)q.c.seqs * d->Hkv * pl.chunks * 16 <= pl.grid;
+    e = few ? launch_pdl<true>(decode_join_kernel<T, D, NT, 1>, dim3(pl.grid, Cfg::HEADS), dim3(JOIN_THREADS), 0, stream, q)
+            : launch_pdl<true>(decode_join_kernel<T, D, NT, 8>, dim3(pl.grid, NT), dim3(JOIN_THREADS), 0, stream, q);
+    if (e != cudaSuccess) return INCIN_ERR_LAUNCH;
   }
   return INCIN_OK;
 }
