@@ -567,9 +567,9 @@ static EncodeTiledFn get_encode() {
 }
 
 // Tensor map over a bf16 operand: dims {inner, rows, batch_lo, batch_hi}, strides in elements.
-int make_operand_map(CUtensorMap* out, const void* ptr, long long inner, long long rows, long long ld,
-                     long long batch_lo, long long stride_lo, long long batch_hi, long long stride_hi, int box_inner,
-                     int box_rows) {
+int make_operand_map_box(CUtensorMap* out, const void* ptr, long long inner, long long rows, long long ld,
+                         long long batch_lo, long long stride_lo, long long batch_hi, long long stride_hi, int box_inner,
+                         int box_rows, int box_lo) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return INCIN_ERR_DRIVER;
   // cuTensorMapEncodeTiled is a driver call and needs a current context on the calling thread.  Autograd
@@ -586,12 +586,17 @@ int make_operand_map(CUtensorMap* out, const void* ptr, long long inner, long lo
   // strides of dims 1..3 in bytes; a unit batch dimension still needs a legal (multiple of 16) stride
   cuuint64_t strides[3] = {(cuuint64_t)ld * 2, (cuuint64_t)(batch_lo > 1 ? stride_lo : ld * rows) * 2,
                            (cuuint64_t)(batch_hi > 1 ? stride_hi : ld * rows) * 2};
-  cuuint32_t box[4] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_lo, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? INCIN_OK : INCIN_ERR_TENSOR_MAP;
+}
+int make_operand_map(CUtensorMap* out, const void* ptr, long long inner, long long rows, long long ld,
+                     long long batch_lo, long long stride_lo, long long batch_hi, long long stride_hi, int box_inner,
+                     int box_rows) {
+  return make_operand_map_box(out, ptr, inner, rows, ld, batch_lo, stride_lo, batch_hi, stride_hi, box_inner, box_rows, 1);
 }
 
 // Tensor map over an fp32 tensor for tiled reduce-adds from 128-byte swizzled shared memory: dims {inner, rows,

@@ -1,0 +1,728 @@
+// Causal attention of packed runs of new tokens over a paged key-value cache.
+//
+// One persistent CTA per SM works on items: up to two 128-row query tiles of one sequence and key head, over a range of its
+// keys.  The rows of a tile are (new token, query head of the key head), so that grouped heads share every key that is
+// loaded and a run of a few tokens still fills a tile: with G query heads a key head a tile holds 128 / G tokens.  A box of
+// the query map is {64 elements, G heads, 128 / G tokens}, one copy a half.  K and V tiles are 128 keys, fetched page
+// by page (a box is one page of one head); the lanes of the producer warp hold the page numbers.
+//
+// The arithmetic and its schedule are those of the dense causal kernel (attention_fwd.cu): S_w = Q_w K^T into tensor memory, a
+// softmax thread a row, P_w over S_w's columns, O_w += P_w V from tensor memory, the other tile's products meanwhile.  What
+// is different here:
+// - Items come from lengths that only the device knows.  The producer warp walks the sequences, 32 at a time by a scan
+//   across its lanes, and hands items to the other warps through a ring.
+// - Few rows over many keys: the keys of an item are split among `splits` CTAs, which leave fp32 parts (O, m, l) that a second
+//   kernel joins in a fixed order.
+// - The last page of a sequence has slots without tokens, and a tile's keys go past its first rows' own positions.  Scores
+//   there are replaced by -inf, but P = 0 times a NaN or an infinity in V would still be NaN.  So two warps look over the V
+//   tiles that hold such keys before the product reads them: rows behind the sequence become zeros, and non-finite
+//   elements of keys that some row must not see become zeros and are added back, row by row, at the end (an item that had
+//   any reads them from the cache again; a weight is positive, so the element itself is what the sum takes from it).
+#include "paged.cuh"
+
+#include <math_constants.h>
+
+namespace incin {
+
+int make_operand_map(CUtensorMap* out, const void* ptr, long long inner, long long rows, long long ld, long long batch_lo,
+                     long long stride_lo, long long batch_hi, long long stride_hi, int box_inner, int box_rows);
+int make_operand_map_box(CUtensorMap* out, const void* ptr, long long inner, long long rows, long long ld, long long batch_lo,
+                         long long stride_lo, long long batch_hi, long long stride_hi, int box_inner, int box_rows, int box_lo);
+
+constexpr int PR_BM = 128;        // rows of a query tile, keys of a K / V tile
+constexpr int PR_THREADS = 384;   // warp 0: items and TMA, 1: tcgen05 issue, 2-3: V tiles, 4-7 / 8-11: softmax of tile 0 / 1
+// 384 threads are launched with 168 registers each: 128 x (88 + 208 + 208) = 64512
+constexpr int PR_REGS_ISSUE = 88, PR_REGS_SOFTMAX = 208;
+constexpr int PR_ITEMS = 3;       // slots of the item ring
+
+template <int D>
+struct PrCfg {
+  static constexpr int TILE_BYTES = PR_BM * D * 2;
+  static constexpr int STAGES = D == 128 ? 5 : 8;       // ring of K V K V ... tiles
+  static constexpr int OFF_RING = 2 * TILE_BYTES;
+  static constexpr int OFF_BAR = OFF_RING + STAGES * TILE_BYTES;
+  static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;
+  // tensor memory: S_w (P_w in its first 64 columns) at [128 w, 128 w + 128), O_w at 256 + D w
+  static constexpr int TMEM_COLS = 512, COL_O = 256;
+  static constexpr int PART = 96;   // columns of P_w after which the first products of O_w += P_w V are let go
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared-memory plan");
+};
+
+struct PrItem {
+  int seq, head;     // key head; -1 ends the list
+  int row0, tokens;  // first packed row of tile 0, new tokens from there to the end of the sequence's run
+  int pos0;          // position of that token (negative: more new tokens than the sequence has)
+  int length;        // tokens of the sequence
+  int lo, hi[2];     // K / V tiles [lo, hi[w]) for tile w
+  int split;
+  int odd;           // set when a non-finite element of a late key was taken out of a V tile
+};
+
+struct PrParams {
+  PagedView c;
+  uint16_t* out;
+  float scale_log2;
+  int group, tokens;   // query heads of a key head, tokens of a tile
+  int tiles;           // query tiles of an item: 2, or 1 where twice as many items are wanted
+  int splits;
+  float* part_o;       // [splits][rows][Hq][D]
+  float2* part_ml;     // [splits][rows][Hq]: m and l; l = -1 for a row without a position
+};
+
+template <typename T>
+struct PrType;
+template <>
+struct PrType<Bf16> {
+  static constexpr uint32_t FORMAT = 1, EXPONENT = 0x7f807f80u;
+};
+template <>
+struct PrType<Fp16> {
+  static constexpr uint32_t FORMAT = 0, EXPONENT = 0x7c007c00u;
+};
+// Whether either half of a word is an infinity or NaN: its exponent bits are all ones.
+template <typename T>
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+  return __vcmpeq2(w & PrType<T>::EXPONENT, PrType<T>::EXPONENT) != 0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PR_THREADS, 1)
+prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const PrParams p) {
+  using Cfg = PrCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sRing = smem + Cfg::OFF_RING;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* full = bars;              // [STAGES <= 8] a K or V tile has landed
+  uint64_t* empty = bars + 8;         // [STAGES <= 8] the products that read it have finished
+  uint64_t* clean = bars + 16;        // [STAGES <= 8] a V tile has been looked over (two warps)
+  uint64_t* q_full = bars + 24;       // [2] query tile w has landed
+  uint64_t* q_empty = bars + 26;      // [2] the last score product of query tile w has finished
+  uint64_t* s_full = bars + 28;       // [2] S_w is in tensor memory (and every earlier product has finished)
+  uint64_t* p_full = bars + 30;       // [2] P_w is in tensor memory, O_w rescaled
+  uint64_t* o_full = bars + 32;       // [2] O_w of this item is complete
+  uint64_t* p_part = bars + 34;       // [2] the first PART columns of P_w are in tensor memory
+  uint64_t* item_full = bars + 36;    // [PR_ITEMS]
+  uint64_t* item_empty = bars + 40;   // [PR_ITEMS] one arrival a warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  PrItem* items = reinterpret_cast<PrItem*>(bars + 46);   // [PR_ITEMS]
+
+  const PagedView& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&clean[s], 2);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&q_empty[w], 1);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 4);
+      mbar_init(&o_full[w], 1);
+      mbar_init(&p_part[w], 4);
+    }
+    for (int i = 0; i < PR_ITEMS; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);   // every warp but the producer
+    }
+    *abort_flag = 0;
+    mbar_init_fence();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();   // tensor memory is held; a successor may be scheduled as CTAs retire
+  pdl_wait();                // no global memory was touched above
+
+  // The next item, for every warp but the producer: returned by value, `slot` kept until the warp lets go of it.
+  auto take_item = [&](int i, PrItem& it) -> bool {
+    const int slot = i % PR_ITEMS;
+    if (!mbar_wait(&item_full[slot], (i / PR_ITEMS) & 1, abort_flag, c.status, kStatusTimeoutFull)) return false;
+    it = items[slot];
+    return it.head >= 0;
+  };
+  auto drop_item = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[i % PR_ITEMS]);
+  };
+  // Keys from this one on are not seen by every row of the item.
+  auto late_from = [&](const PrItem& it) { return it.pos0 + 1; };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_ISSUE));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- items and loads; warp-uniform, lanes issue copies
+      const bool leader = elect_one() != 0;
+      int stage = 0;
+      uint32_t phase = 0, q_phase[2] = {0, 0};
+      bool ok = true;
+      const int per_tile = PR_BM >> c.page_shift;   // pages of a K / V tile
+      // sequences [chunk, chunk + 32): a lane's items and those in front of them
+      int chunk = -32, before = 0, total = 0, my_items = 0, my_upto = 0, my_row = 0, my_new = 0, my_len = 0;
+      const int item_tokens = p.tiles * p.tokens;
+      for (int i = 0; ok; ++i) {
+        const int G = (int)gridDim.x, cta = (int)blockIdx.x;
+        const int idx = (i & 1) ? (i + 1) * G - 1 - cta : i * G + cta;   // snake order: long and short items in turn
+        while (chunk < c.seqs && idx >= before + total) {
+          chunk += 32;
+          before += total;
+          const int s = chunk + lane;
+          my_items = my_row = my_new = my_len = 0;
+          if (s < c.seqs) {
+            my_row = min(max(c.offsets[s], 0), c.rows);
+            my_new = min(max(c.offsets[s + 1], my_row), c.rows) - my_row;
+            my_len = paged_length(c, s);
+            if (my_new > my_len) flag_bad_index(c.status);
+            my_items = (my_new + item_tokens - 1) / item_tokens * c.Hkv * p.splits;
+          }
+          my_upto = my_items;
+#pragma unroll
+          for (int w = 1; w < 32; w <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, my_upto, w);
+            if (lane >= w) my_upto += other;
+          }
+          total = __shfl_sync(0xffffffffu, my_upto, 31);
+        }
+        PrItem it = {};
+        it.head = -1;
+        if (chunk < c.seqs) {
+          const int at = idx - before;
+          const int owner = __ffs(__ballot_sync(0xffffffffu, at < my_upto)) - 1;
+          const int first = __shfl_sync(0xffffffffu, my_upto - my_items, owner), runs = __shfl_sync(0xffffffffu, my_items, owner);
+          const int row = __shfl_sync(0xffffffffu, my_row, owner), fresh = __shfl_sync(0xffffffffu, my_new, owner);
+          it.length = __shfl_sync(0xffffffffu, my_len, owner);
+          it.seq = chunk + owner;
+          const int per = c.Hkv * p.splits, rest = at - first;
+          const int pair = runs / per - 1 - rest / per, k = rest % per;   // the longest first
+          it.head = k / p.splits;
+          it.split = k % p.splits;
+          const int t0 = pair * item_tokens;
+          it.row0 = row + t0;
+          it.tokens = fresh - t0;
+          it.pos0 = it.length - fresh + t0;
+          int n[2];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {   // tiles up to the last row's own position
+            const int last = it.pos0 + min((w + 1) * p.tokens, it.tokens) - 1;
+            n[w] = w < p.tiles && w * p.tokens < it.tokens && last >= 0 ? last / PR_BM + 1 : 0;
+          }
+          const int most = max(n[0], n[1]);
+          it.lo = (int)((long long)most * it.split / p.splits);
+          const int hi = (int)((long long)most * (it.split + 1) / p.splits);
+          it.hi[0] = min(hi, n[0]);
+          it.hi[1] = min(hi, n[1]);
+        }
+        const int slot = i % PR_ITEMS;
+        if (!mbar_wait(&item_empty[slot], ((i / PR_ITEMS) & 1) ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) break;
+        if (lane == 0) {
+          items[slot] = it;
+          mbar_arrive(&item_full[slot]);
+        }
+        __syncwarp();
+        if (it.head < 0) break;
+
+        const int hi = max(it.hi[0], it.hi[1]);
+        const int entries = (it.length + (1 << c.page_shift) - 1) >> c.page_shift;   // pages with tokens
+        auto load_q = [&](int w) -> bool {
+          if (!mbar_wait(&q_empty[w], q_phase[w] ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) return false;
+          q_phase[w] ^= 1;
+          if (leader) {
+            mbar_expect_tx(&q_full[w], p.group * p.tokens * D * 2);
+#pragma unroll
+            for (int ch = 0; ch < D / 64; ++ch)
+              tma_load_4d(smem + w * Cfg::TILE_BYTES + ch * (PR_BM * 128), &tmQ, &q_full[w], ch * 64, it.head * p.group, it.row0 + w * p.tokens, 0);
+          }
+          __syncwarp();
+          return true;
+        };
+        // a lane holds one of the next 32 page numbers; `pages` (out of range: zeros are filled in) where there is none
+        int held_from = it.lo * per_tile, held;
+        auto hold = [&](int from) {
+          const int e = from + lane;
+          const int page = e < entries ? paged_page(c, it.seq, e) : -1;
+          return page < 0 ? c.pages : page;
+        };
+        held = hold(held_from);
+        int ahead = hold(held_from + 32);
+        auto load_kv = [&](const CUtensorMap* tm, int j) -> bool {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) return false;
+          if (leader) mbar_expect_tx(&full[stage], Cfg::TILE_BYTES);
+          __syncwarp();
+          const int box = lane % per_tile, ch = lane / per_tile;
+          const int page = __shfl_sync(0xffffffffu, held, j * per_tile - held_from + box);
+          if (ch < D / 64)
+            tma_load_4d(sRing + stage * Cfg::TILE_BYTES + ch * (PR_BM * 128) + (box << c.page_shift) * 128, tm, &full[stage], ch * 64, 0, it.head, page);
+          __syncwarp();
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+          return true;
+        };
+        if (hi > it.lo) {
+          bool first_q = it.hi[0] > it.lo, second_q = it.hi[1] > it.lo;
+          for (int j = it.lo; j < hi && ok; ++j) {
+            if (j * per_tile >= held_from + 32) {
+              held = ahead;
+              held_from += 32;
+              ahead = hold(held_from + 32);
+            }
+            if (first_q) ok = load_q(0);
+            ok = ok && load_kv(&tmK, j);
+            if (second_q) ok = ok && load_q(1);
+            ok = ok && load_kv(&tmV, j);
+            first_q = second_q = false;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- products: one elected lane issues.  S_w(j+1) follows
+      // O_w += P_w(j) V_j although it overwrites P_w: products of one issuing thread run in order (see attention_fwd.cu).
+      const bool leader = elect_one() != 0;
+      constexpr uint32_t idesc_s = idesc_with_format(make_idesc_bf16(PR_BM, PR_BM, false, false), PrType<T>::FORMAT);
+      constexpr uint32_t idesc_o = idesc_with_format(make_idesc_bf16(PR_BM, D, false, true), PrType<T>::FORMAT);
+      constexpr uint32_t kDescHi = ((1024u >> 4) & 0x3FFF) | (1u << 14) | (2u << 29);   // SBO 1024, version, SWIZZLE_128B
+      constexpr uint32_t kLoK = (16u >> 4) << 16;                                       // K-major: LBO 16
+      constexpr uint32_t kLoMN = ((uint32_t)(PR_BM * 128) >> 4) << 16;                  // MN-major V: 64-column chunks 16 KB apart
+      auto desc = [&](uint32_t lo) -> uint64_t { return (static_cast<uint64_t>(kDescHi) << 32) | lo; };
+      const uint32_t q16 = (smem_u32(smem) & 0x3FFFF) >> 4, ring16 = (smem_u32(sRing) & 0x3FFFF) >> 4;
+      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, clean_phase = 0;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      auto scores = [&](int w, int k_stage) {   // S_w = Q_w K^T
+        const uint32_t a = q16 + w * (Cfg::TILE_BYTES >> 4), bk = ring16 + k_stage * (Cfg::TILE_BYTES >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (PR_BM * 128 >> 4) + (kk & 3) * 2;
+          if (leader) umma_f16_ss(tmem_base + w * PR_BM, desc(a + off + kLoK), desc(bk + off + kLoK), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        if (leader) umma_commit(&s_full[w]);
+        __syncwarp();
+      };
+      auto take = [&](int& my_stage) -> bool {   // next tile of the ring
+        if (!mbar_wait(&full[stage], phase, abort_flag, c.status, kStatusTimeoutFull)) return false;
+        my_stage = stage;
+        if (++stage == Cfg::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+        return true;
+      };
+      PrItem it;
+      for (int i = 0; ok && take_item(i, it); ++i) {
+        const int lo = it.lo, hi = max(it.hi[0], it.hi[1]);
+        if (hi > lo) {
+          int k_stage = 0, v_stage = 0;
+          ok = take(k_stage);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (!ok || it.hi[w] <= lo) continue;
+            ok = mbar_wait(&q_full[w], q_phase[w], abort_flag, c.status, kStatusTimeoutFull);
+            if (!ok) continue;
+            q_phase[w] ^= 1;
+            tc_fence_after();
+            scores(w, k_stage);
+            if (leader && it.hi[w] == lo + 1) umma_commit(&q_empty[w]);
+          }
+          if (ok && leader) umma_commit(&empty[k_stage]);
+          for (int j = lo; j < hi && ok; ++j) {
+            ok = take(v_stage);
+            if (ok) {
+              ok = mbar_wait(&clean[v_stage], (clean_phase >> v_stage) & 1, abort_flag, c.status, kStatusTimeoutFull);
+              clean_phase ^= 1u << v_stage;
+            }
+            if (ok && j + 1 < hi) ok = take(k_stage);
+            if (!ok) break;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (!ok || j >= it.hi[w]) continue;
+              const uint32_t bv = ring16 + v_stage * (Cfg::TILE_BYTES >> 4);
+              // O_w += P_w V: 16 keys per product, P_w from tensor memory, the first products before all of P_w is there
+              ok = mbar_wait(&p_part[w], p_phase[w], abort_flag, c.status, kStatusTimeoutTmemFull);
+              if (!ok) continue;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < PR_BM / 16; ++kk) {
+                if (kk == Cfg::PART / 16) {
+                  ok = mbar_wait(&p_full[w], p_phase[w], abort_flag, c.status, kStatusTimeoutTmemFull);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                if (leader) umma_f16_ts(tmem_base + Cfg::COL_O + w * D, tmem_base + w * PR_BM + kk * 8, desc(bv + kk * 128 + kLoMN), idesc_o,
+                                        (j > lo || kk > 0) ? 1u : 0u);
+              }
+              if (!ok) continue;
+              p_phase[w] ^= 1;
+              if (j + 1 < it.hi[w]) {
+                scores(w, k_stage);
+                if (leader && j + 2 == it.hi[w]) umma_commit(&q_empty[w]);
+              } else if (leader) {
+                umma_commit(&o_full[w]);
+              }
+              __syncwarp();
+            }
+            if (ok && leader) {
+              umma_commit(&empty[v_stage]);
+              if (j + 1 < hi) umma_commit(&empty[k_stage]);
+            }
+            __syncwarp();
+          }
+        }
+        drop_item(i);
+      }
+    } else {
+      // ---------------------------------------------------------------- V tiles with late keys: 64 threads, two rows each
+      const int tid = (warp - 2) * 32 + lane;
+      int stage = 0;   // ring position of the item's next K tile
+      uint32_t phase = 0;
+      bool ok = true;
+      PrItem it;
+      // rows outside every sequence give zeros
+      {
+        const int begin = min(max(c.offsets[0], 0), c.rows), end = min(max(c.offsets[c.seqs], begin), c.rows);
+        const long long row_vecs = (long long)c.Hq * (D / 8), outside = (long long)(begin + c.rows - end) * row_vecs;
+        for (long long i = (long long)blockIdx.x * 64 + tid; i < outside; i += (long long)gridDim.x * 64) {
+          const long long r = i / row_vecs, row = r < begin ? r : end + (r - begin);
+          reinterpret_cast<uint4*>(p.out)[row * row_vecs + i % row_vecs] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      for (int i = 0; ok && take_item(i, it); ++i) {
+        const int hi = max(it.hi[0], it.hi[1]), late = late_from(it);
+        for (int j = it.lo; j < hi && ok; ++j) {
+          int v_stage = stage + 1;
+          uint32_t v_phase = phase;
+          if (v_stage == Cfg::STAGES) {
+            v_stage = 0;
+            v_phase ^= 1;
+          }
+          stage = v_stage + 1;
+          phase = v_phase;
+          if (stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+          // every V tile passes through here, so that these warps keep step with the ring
+          ok = mbar_wait(&full[v_stage], v_phase, abort_flag, c.status, kStatusTimeoutFull);
+          if (!ok) break;
+          if ((j + 1) * PR_BM <= late) {
+            if (lane == 0) mbar_arrive(&clean[v_stage]);
+            continue;
+          }
+          uint8_t* tile = sRing + v_stage * Cfg::TILE_BYTES;
+#pragma unroll 1
+          for (int row = tid; row < PR_BM; row += 64) {
+            const int key = j * PR_BM + row;
+            if (key < late) continue;
+            auto vec = [&](int ch, int u) { return reinterpret_cast<uint4*>(tile + ch * (PR_BM * 128) + row * 128 + ((u ^ (row & 7)) << 4)); };
+            if (key >= it.length) {
+#pragma unroll
+              for (int u = 0; u < D / 8; ++u) *vec(u >> 3, u & 7) = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            bool odd = false;
+#pragma unroll
+            for (int u = 0; u < D / 8; ++u) {
+              const uint4 x = *vec(u >> 3, u & 7);
+              odd |= odd_word<T>(x.x) || odd_word<T>(x.y) || odd_word<T>(x.z) || odd_word<T>(x.w);
+            }
+            if (odd) {
+              items[i % PR_ITEMS].odd = 1;
+              for (int u = 0; u < D / 8; ++u) {
+                uint4 x = *vec(u >> 3, u & 7);
+                uint32_t* xs = &x.x;
+                for (int e = 0; e < 4; ++e) xs[e] &= ~__vcmpeq2(xs[e] & PrType<T>::EXPONENT, PrType<T>::EXPONENT);
+                *vec(u >> 3, u & 7) = x;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&clean[v_stage]);
+        }
+        drop_item(i);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
+    // ------------------------------------------------------------------ softmax / rescale / epilogue of query tile w
+    const int w = (warp >> 2) - 1;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // row inside the tile == TMEM lane
+    const int token = row / p.group, g = row - token * p.group;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tmem_S = tmem_base + w * PR_BM + lane_addr, tmem_O = tmem_base + Cfg::COL_O + w * D + lane_addr;
+    uint32_t s_phase = 0, o_phase = 0;
+    bool ok = true;
+    PrItem it;
+    for (int i = 0; ok && take_item(i, it); ++i) {
+      const int lo = it.lo, hi = it.hi[w];
+      const int mine = w * p.tokens + token;                     // token of the item
+      const bool live_row = w < p.tiles && token < p.tokens && mine < it.tokens;
+      const int limit = it.pos0 + (live_row ? mine : min(w * p.tokens, it.tokens - 1));   // the last key that the row sees
+      const int all_see = it.pos0 + w * p.tokens;                // ... and the last one that every row of the tile sees
+      float m_ref = -CUDART_INF_F;
+      float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      for (int j = lo; j < hi; ++j) {
+        if (!mbar_wait(&s_full[w], s_phase, abort_flag, c.status, kStatusTimeoutTmemFull)) { ok = false; break; }
+        s_phase ^= 1;
+        tc_fence_after();
+        // whole S row into registers with back-to-back TMEM loads and a single wait
+        uint32_t s[PR_BM];
+#pragma unroll
+        for (int ch = 0; ch < PR_BM / 32; ++ch) tmem_ld_32x32(tmem_S + ch * 32, reinterpret_cast<uint32_t(&)[32]>(s[ch * 32]));
+        tmem_ld_wait();
+        if (j * PR_BM + PR_BM - 1 > all_see) {   // masked scores become -inf
+          const int last = limit - j * PR_BM;
+#pragma unroll
+          for (int e = 0; e < PR_BM; ++e)
+            if (e > last) s[e] = __float_as_uint(-CUDART_INF_F);
+        }
+        float mx4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};   // four chains, three-input maxima
+#pragma unroll
+        for (int e = 0; e < PR_BM; e += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(fmaxf(mx4[k], __uint_as_float(s[e + k * 2])), __uint_as_float(s[e + k * 2 + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        // lazy rescale: only move the reference when the maximum grew by more than 2^8
+        const bool need = mx > m_ref + 8.0f;
+        if (__any_sync(0xffffffffu, need)) {
+          const float alpha = need ? exp2f(m_ref - mx) : 1.0f;   // 0 the first time
+          if (need) m_ref = mx;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            l2[e].x *= alpha;
+            l2[e].y *= alpha;
+          }
+          if (j > lo) {   // s_full covers O_w += P_w(j-1) V_{j-1}: O_w is at rest
+#pragma unroll 1
+            for (int ch = 0; ch < D / 32; ++ch) {
+              uint32_t o[32];
+              tmem_ld_32x32(tmem_O + ch * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_32x32(tmem_O + ch * 32, o);
+            }
+          }
+        }
+        // P = exp2(s * scale - m_ref) in the cache's type over the first half of S_w's columns, row sums in fp32; a row that
+        // has only seen scores of -inf weighs them 0
+        const float ref = m_ref == -CUDART_INF_F ? 0.f : -m_ref;
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(ref, ref);
+#pragma unroll
+        for (int ch = 0; ch < PR_BM / 32; ++ch) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(s[ch * 32 + e]), __uint_as_float(s[ch * 32 + e + 1])), sc2, nm2);
+            const float2 y = make_float2(exp2f(x.x), exp2f(x.y));
+            l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], y);
+            pk[e >> 1] = T::pack(y.x, y.y);
+          }
+          tmem_st_32x16(tmem_S + ch * 16, pk);
+          if ((ch + 1) * 32 == Cfg::PART) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_part[w]);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();                        // every lane's stores and fences precede the single arrival of its warp
+        if (lane == 0) mbar_arrive(&p_full[w]);
+      }
+      const bool ran = hi > lo;
+      if (ran) {
+        if (!ok || !mbar_wait(&o_full[w], o_phase, abort_flag, c.status, kStatusTimeoutTmemFull)) { ok = false; break; }
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+      const float l_sum = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+      const long long out_row = (long long)(it.row0 + mine) * c.Hq + it.head * p.group + g;
+      const bool odd = ran && *reinterpret_cast<volatile int*>(&items[i % PR_ITEMS].odd);
+      const bool parts = p.splits > 1;
+      const float inv = limit < 0 ? 0.f : parts ? 1.f : 1.0f / l_sum;
+#pragma unroll 1
+      for (int ch = 0; ch < D / 32; ++ch) {
+        uint32_t o[32];
+        if (ran) {
+          tmem_ld_32x32(tmem_O + ch * 32, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+        if (odd && live_row) {   // non-finite elements of late keys, left out of the products
+          for (int key = max(late_from(it), lo * PR_BM); key <= min(limit, hi * PR_BM - 1); ++key) {
+            const int page = paged_page(c, it.seq, key >> c.page_shift);
+            if (page < 0) continue;
+            const uint16_t* v = c.v + page * c.v_page + it.head * c.v_head + (key & ((1 << c.page_shift) - 1)) * c.v_token + ch * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(v + e);
+              const uint32_t bad = __vcmpeq2(x & PrType<T>::EXPONENT, PrType<T>::EXPONENT);
+              const float2 y = T::unpack(x);
+              if (bad & 0xffffu) o[e] = __float_as_uint(__uint_as_float(o[e]) + y.x);
+              if (bad >> 16) o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) + y.y);
+            }
+          }
+        }
+        if (live_row && parts) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + ((long long)it.split * c.rows * c.Hq + out_row) * D + ch * 32);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            dst[u] = make_float4(__uint_as_float(o[u * 4]), __uint_as_float(o[u * 4 + 1]), __uint_as_float(o[u * 4 + 2]), __uint_as_float(o[u * 4 + 3]));
+        } else if (live_row) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = T::pack(__uint_as_float(o[e * 2]), __uint_as_float(o[e * 2 + 1]));
+          uint16_t* dst = p.out + out_row * D + ch * 32;
+          if (aligned32(dst)) {   // 32 bytes per store: whole sectors of the row
+            st_global_b256(dst, reinterpret_cast<uint32_t(&)[8]>(pk[0]));
+            st_global_b256(dst + 16, reinterpret_cast<uint32_t(&)[8]>(pk[8]));
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (live_row && parts) p.part_ml[(long long)it.split * c.rows * c.Hq + out_row] = make_float2(m_ref, limit < 0 ? -1.f : l_sum);
+      tc_fence_before();   // O_w has been read before the next item's first product, which follows this warp's p_part
+      drop_item(i);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// Joins the parts of a row and query head: a warp each.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
+  constexpr int PER = D / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const PagedView& c = p.c;
+  const long long n = (long long)c.rows * c.Hq, at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int begin = min(max(c.offsets[0], 0), c.rows), end = min(max(c.offsets[c.seqs], begin), c.rows);
+  if (at >= n || at / c.Hq < begin || at / c.Hq >= end) return;
+  const float2 ml = lane < p.splits ? p.part_ml[lane * n + at] : make_float2(-CUDART_INF_F, 0.f);
+  float top = ml.x;
+#pragma unroll
+  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  const float weight = ml.x == -CUDART_INF_F ? 0.f : ml.x == top ? 1.f : exp2f(ml.x - top);
+  const bool nowhere = __any_sync(0xffffffffu, ml.y < 0.f);
+  float sum = weight * ml.y, acc[PER] = {};
+#pragma unroll
+  for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+#pragma unroll 4
+  for (int i = 0; i < p.splits; ++i) {
+    const float f = __shfl_sync(0xffffffffu, weight, i);
+    if (f == 0.f) continue;
+    const float* src = p.part_o + (i * n + at) * D + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] += f * src[e];
+  }
+  const float inv = nowhere ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(p.out + at * D + lane * PER)[e / 2] = T::pack(acc[e] * inv, acc[e + 1] * inv);
+}
+
+struct PrPlan {
+  int tokens, tiles, splits;
+  long long items, bytes;
+};
+
+static PrPlan pr_plan(const incin_paged_desc* d) {
+  PrPlan pl;
+  const int sms = device_sm_count();
+  pl.tokens = PR_BM / (d->Hq / d->Hkv);
+  auto items = [&](int tiles) { return ((long long)d->rows / (tiles * pl.tokens) + d->seqs) * d->Hkv; };   // at most
+  pl.tiles = 2;
+  pl.splits = 1;
+  if (items(1) <= sms) pl.tiles = 1;
+  // keys of a sequence at most, in tiles
+  const long long keys = ((long long)d->table_width * d->page_size + PR_BM - 1) / PR_BM;
+  const long long n = ((long long)d->rows + pl.tiles * pl.tokens - 1) / (pl.tiles * pl.tokens) * d->Hkv;
+  if (n * 2 <= sms) {
+    long long s = sms / n;
+    if (s > keys / 4) s = keys / 4;
+    pl.splits = s < 1 ? 1 : s > 32 ? 32 : (int)s;
+  }
+  pl.items = items(pl.tiles) * pl.splits;
+  pl.bytes = pl.splits > 1 ? (long long)pl.splits * d->rows * d->Hq * (d->D * 4 + 8) : 0;
+  return pl;
+}
+
+template <typename T, int D>
+static int launch_prompt(const incin_paged_desc* d, cudaStream_t stream) {
+  using Cfg = PrCfg<D>;
+  const PrPlan pl = pr_plan(d);
+  if (pl.items > (1ll << 30)) return INCIN_ERR_TOO_LARGE;   // the kernel counts items in 32 bits
+  if (pl.bytes && !d->workspace) return INCIN_ERR_ARGUMENT;
+  const int group = d->Hq / d->Hkv;
+  CUtensorMap tq, tk, tv;
+  int rc = make_operand_map_box(&tq, d->x, D, d->Hq, d->Hq > 1 ? d->x_stride_head : D, d->rows, d->x_stride_row, 1, 0, 64, group, pl.tokens);
+  if (rc) return rc;
+  rc = make_operand_map(&tk, d->k_pages, D, d->page_size, d->k_stride_token, d->Hkv, d->k_stride_head, d->pages, d->k_stride_page, 64, d->page_size);
+  if (rc) return rc;
+  rc = make_operand_map(&tv, d->v_pages, D, d->page_size, d->v_stride_token, d->Hkv, d->v_stride_head, d->pages, d->v_stride_page, 64, d->page_size);
+  if (rc) return rc;
+  auto kern = prompt_attention_kernel<T, D>;
+  static PerDeviceFlags attr;
+  if (!ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr)) return INCIN_ERR_LAUNCH;
+  const long long n = (long long)d->rows * d->Hq;
+  const PrParams p = {paged_view(d), (uint16_t*)d->out, d->scale * 1.4426950408889634f, group, pl.tokens, pl.tiles, pl.splits,
+                      (float*)d->workspace, (float2*)((float*)d->workspace + pl.splits * n * D)};
+  const int sms = device_sm_count();
+  if (launch_pdl<true>(kern, dim3((unsigned)(pl.items < sms ? pl.items : sms)), dim3(PR_THREADS), Cfg::SMEM_BYTES, stream, tq, tk, tv, p) != cudaSuccess)
+    return INCIN_ERR_LAUNCH;
+  if (pl.splits > 1 &&
+      launch_pdl<true>(prompt_join_kernel<T, D>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, stream, p) != cudaSuccess)
+    return INCIN_ERR_LAUNCH;
+  return INCIN_OK;
+}
+
+}  // namespace incin
+
+extern "C" long long incin_prompt_attention_workspace(const incin_paged_desc* d) {
+  if (!d || d->Hkv <= 0 || d->Hq < d->Hkv || d->Hq / d->Hkv > 128) return 0;
+  return incin::pr_plan(d).bytes;
+}
+
+extern "C" int incin_prompt_attention(const incin_paged_desc* d, void* stream) {
+  using namespace incin;
+  const int rc = check_paged(d);
+  if (rc) return rc;
+  if (!d->offsets) return INCIN_ERR_ARGUMENT;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (d->dtype == INCIN_GEMM_IN_FP16) return d->D == 64 ? launch_prompt<Fp16, 64>(d, s) : launch_prompt<Fp16, 128>(d, s);
+  return d->D == 64 ? launch_prompt<Bf16, 64>(d, s) : launch_prompt<Bf16, 128>(d, s);
+}
