@@ -105,9 +105,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* p_part = bars + 34;       // [2] the first PART columns of P_w are in tensor memory
   uint64_t* item_full = bars + 36;    // [PR_ITEMS]
   uint64_t* item_empty = bars + 40;   // [PR_ITEMS] one arrival a warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
+  uint64_t* stolen = bars + 43;       // the answer about the next item has landed
+  uint4* answer = reinterpret_cast<uint4*>(bars + 44);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  PrItem* items = reinterpret_cast<PrItem*>(bars + 46);   // [PR_ITEMS]
+  PrItem* items = reinterpret_cast<PrItem*>(bars + 48);   // [PR_ITEMS]
 
   const PagedView& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -126,6 +128,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(&o_full[w], 1);
       mbar_init(&p_part[w], 4);
     }
+    mbar_init(stolen, 1);
     for (int i = 0; i < PR_ITEMS; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 11);   // every warp but the producer
@@ -173,10 +176,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       // sequences [chunk, chunk + 32): a lane's items and those in front of them
       int chunk = -32, before = 0, total = 0, my_items = 0, my_upto = 0, my_row = 0, my_new = 0, my_len = 0;
       const int item_tokens = p.tiles * p.tokens;
-      for (int i = 0; ok; ++i) {
-        const int G = (int)gridDim.x, cta = (int)blockIdx.x;
-        const int idx = (i & 1) ? (i + 1) * G - 1 - cta : i * G + cta;   // snake order: long and short items in turn
-        while (chunk < c.seqs && idx >= before + total) {
+      // An item per CTA of the grid; CTAs that run take over those that have not started.
+      int idx = (int)blockIdx.x;
+      uint32_t steal_phase = 0;
+      int published = 0;
+      while (ok) {
+        if (idx >= 0 && idx < before) chunk = -32, before = total = 0;   // (indices come in rising order)
+        while (idx >= 0 && chunk < c.seqs && idx >= before + total) {
           chunk += 32;
           before += total;
           const int s = chunk + lane;
@@ -198,7 +204,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         PrItem it = {};
         it.head = -1;
-        if (chunk < c.seqs) {
+        const bool there = idx >= 0 && chunk < c.seqs;   // the grid has an index for every item that there could be
+        if (there) {
           const int at = idx - before;
           const int owner = __ffs(__ballot_sync(0xffffffffu, at < my_upto)) - 1;
           const int first = __shfl_sync(0xffffffffu, my_upto - my_items, owner), runs = __shfl_sync(0xffffffffu, my_items, owner);
@@ -225,15 +232,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           it.hi[0] = min(hi, n[0]);
           it.hi[1] = min(hi, n[1]);
         }
-        const int slot = i % PR_ITEMS;
-        if (!mbar_wait(&item_empty[slot], ((i / PR_ITEMS) & 1) ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) break;
-        if (lane == 0) {
-          items[slot] = it;
-          mbar_arrive(&item_full[slot]);
+        if (there || idx < 0) {
+          const int slot = published % PR_ITEMS;
+          if (!mbar_wait(&item_empty[slot], ((published / PR_ITEMS) & 1) ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) break;
+          if (lane == 0) {
+            items[slot] = it;
+            mbar_arrive(&item_full[slot]);
+          }
+          ++published;
+          __syncwarp();
         }
-        __syncwarp();
-        if (it.head < 0) break;
-
+        if (idx < 0) break;
+        auto steal = [&]() {
+          if (leader) {
+            mbar_expect_tx(stolen, 16);
+            steal_cta(answer, stolen);
+          }
+          __syncwarp();
+        };
         const int hi = max(it.hi[0], it.hi[1]);
         const int entries = (it.length + (1 << c.page_shift) - 1) >> c.page_shift;   // pages with tokens
         auto load_q = [&](int w) -> bool {
@@ -272,9 +288,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
           return true;
         };
+        if (hi - it.lo <= 2) steal();
         if (hi > it.lo) {
           bool first_q = it.hi[0] > it.lo, second_q = it.hi[1] > it.lo;
           for (int j = it.lo; j < hi && ok; ++j) {
+            if (j == hi - 2 && j > it.lo) steal();   // late, so that who is done first takes the next item
             if (j * per_tile >= held_from + 32) {
               held = ahead;
               held_from += 32;
@@ -287,6 +305,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             first_q = second_q = false;
           }
         }
+        ok = ok && mbar_wait(stolen, steal_phase, abort_flag, c.status, kStatusTimeoutFull);
+        steal_phase ^= 1;
+        if (ok) idx = stolen_cta(answer);
+        fence_proxy_async_smem();   // the answer has been read before the next one is written
+        __syncwarp();
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- products: one elected lane issues.  S_w(j+1) follows
@@ -701,8 +724,7 @@ static int launch_prompt(const incin_paged_desc* d, cudaStream_t stream) {
   const long long n = (long long)d->rows * d->Hq;
   const PrParams p = {paged_view(d), (uint16_t*)d->out, d->scale * 1.4426950408889634f, group, pl.tokens, pl.tiles, pl.splits,
                       (float*)d->workspace, (float2*)((float*)d->workspace + pl.splits * n * D)};
-  const int sms = device_sm_count();
-  if (launch_pdl<true>(kern, dim3((unsigned)(pl.items < sms ? pl.items : sms)), dim3(PR_THREADS), Cfg::SMEM_BYTES, stream, tq, tk, tv, p) != cudaSuccess)
+  if (launch_pdl<true>(kern, dim3((unsigned)pl.items), dim3(PR_THREADS), Cfg::SMEM_BYTES, stream, tq, tk, tv, p) != cudaSuccess)
     return INCIN_ERR_LAUNCH;
   if (pl.splits > 1 &&
       launch_pdl<true>(prompt_join_kernel<T, D>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, stream, p) != cudaSuccess)

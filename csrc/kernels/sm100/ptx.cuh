@@ -320,6 +320,33 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar_addr) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar_addr)
                : "memory");
 }
+// ---------------------------------------------------------------------------
+// Work stealing among the CTAs of a grid: a running CTA asks for one that has not started yet; if there is one, it never
+// starts, and its index comes back.  The 16-byte answer lands in shared memory and counts 16 bytes on the barrier.  After an
+// answer of "none" the CTA must not ask again.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void steal_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// blockIdx.x of the CTA that was taken over, or -1
+__device__ __forceinline__ int stolen_cta(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n"
+      ".reg .b128 h;\n"
+      ".reg .pred p;\n"
+      "ld.shared.b128 h, [%1];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      "mov.b32 %0, -1;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n"
+      "}\n"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
