@@ -31,16 +31,19 @@ int make_operand_map_box(CUtensorMap* out, const void* ptr, long long inner, lon
 
 constexpr int PR_BM = 128;        // rows of a query tile, keys of a K / V tile
 constexpr int PR_THREADS = 384;   // warp 0: items and TMA, 1: tcgen05 issue, 2-3: V tiles, 4-7 / 8-11: softmax of tile 0 / 1
-// 384 threads are launched with 168 registers each: 128 x (88 + 208 + 208) = 64512
-constexpr int PR_REGS_ISSUE = 88, PR_REGS_SOFTMAX = 208;
+// 384 threads are launched with 168 registers each: 128 x (104 + 200 + 200) = 64512.  (88 and 208: the producer's walk over the
+// sequences spills, 8 runs of 8000 in all, 12 heads of 64, 57.5 us in place of 54.8; 120 and 192: 57.9.)
+constexpr int PR_REGS_ISSUE = 104, PR_REGS_SOFTMAX = 200;
 constexpr int PR_ITEMS = 3;       // slots of the item ring
 
 template <int D>
 struct PrCfg {
   static constexpr int TILE_BYTES = PR_BM * D * 2;
-  static constexpr int STAGES = D == 128 ? 5 : 8;       // ring of K V K V ... tiles
-  static constexpr int OFF_RING = 2 * TILE_BYTES;
-  static constexpr int OFF_BAR = OFF_RING + STAGES * TILE_BYTES;
+  // Rings of K and of V tiles.  They are two because the warps that look over V tiles wait on each of a ring's barriers in
+  // turn: a barrier tells its phases apart by parity alone, so who waits on it has to see every phase.
+  static constexpr int K_STAGES = D == 128 ? 2 : 4, V_STAGES = D == 128 ? 3 : 4;
+  static constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + K_STAGES * TILE_BYTES;
+  static constexpr int OFF_BAR = OFF_V + V_STAGES * TILE_BYTES;
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;
   // tensor memory: S_w (P_w in its first 64 columns) at [128 w, 128 w + 128), O_w at 256 + D w
   static constexpr int TMEM_COLS = 512, COL_O = 256;
@@ -85,6 +88,19 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
   return __vcmpeq2(w & PrType<T>::EXPONENT, PrType<T>::EXPONENT) != 0;
 }
 
+// Position in a ring of N stages.
+template <int N>
+struct PrRing {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(PR_THREADS, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -92,11 +108,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   using Cfg = PrCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sRing = smem + Cfg::OFF_RING;
+  uint8_t *sK = smem + Cfg::OFF_K, *sV = smem + Cfg::OFF_V;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
-  uint64_t* full = bars;              // [STAGES <= 8] a K or V tile has landed
-  uint64_t* empty = bars + 8;         // [STAGES <= 8] the products that read it have finished
-  uint64_t* clean = bars + 16;        // [STAGES <= 8] a V tile has been looked over (two warps)
+  uint64_t *k_full = bars, *v_full = bars + 4;        // [STAGES <= 4] a K or V tile has landed
+  uint64_t *k_empty = bars + 8, *v_empty = bars + 12;   // the products that read it have finished
+  uint64_t* clean = bars + 16;        // [V_STAGES] a V tile has been looked over (two warps)
   uint64_t* q_full = bars + 24;       // [2] query tile w has landed
   uint64_t* q_empty = bars + 26;      // [2] the last score product of query tile w has finished
   uint64_t* s_full = bars + 28;       // [2] S_w is in tensor memory (and every earlier product has finished)
@@ -115,9 +131,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
       mbar_init(&clean[s], 2);
     }
     for (int w = 0; w < 2; ++w) {
@@ -169,8 +187,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     if (warp == 0) {
       // ---------------------------------------------------------------- items and loads; warp-uniform, lanes issue copies
       const bool leader = elect_one() != 0;
-      int stage = 0;
-      uint32_t phase = 0, q_phase[2] = {0, 0};
+      PrRing<Cfg::K_STAGES> k_at;
+      PrRing<Cfg::V_STAGES> v_at;
+      uint32_t q_phase[2] = {0, 0};
       bool ok = true;
       const int per_tile = PR_BM >> c.page_shift;   // pages of a K / V tile
       // sequences [chunk, chunk + 32): a lane's items and those in front of them
@@ -178,6 +197,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int item_tokens = p.tiles * p.tokens;
       // An item per CTA of the grid; CTAs that run take over those that have not started.
       int idx = (int)blockIdx.x;
+      const int begin = min(max(c.offsets[0], 0), c.rows), end = min(max(c.offsets[c.seqs], begin), c.rows);
+      const long long row_vecs = (long long)c.Hq * (D / 8), outside = (long long)(begin + c.rows - end) * row_vecs;
       uint32_t steal_phase = 0;
       int published = 0;
       while (ok) {
@@ -273,19 +294,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         };
         held = hold(held_from);
         int ahead = hold(held_from + 32);
-        auto load_kv = [&](const CUtensorMap* tm, int j) -> bool {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) return false;
-          if (leader) mbar_expect_tx(&full[stage], Cfg::TILE_BYTES);
+        auto load_kv = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* empty, auto& pos, int j) -> bool {
+          if (!mbar_wait(&empty[pos.stage], pos.phase ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) return false;
+          if (leader) mbar_expect_tx(&full[pos.stage], Cfg::TILE_BYTES);
           __syncwarp();
           const int box = lane % per_tile, ch = lane / per_tile;
           const int page = __shfl_sync(0xffffffffu, held, j * per_tile - held_from + box);
           if (ch < D / 64)
-            tma_load_4d(sRing + stage * Cfg::TILE_BYTES + ch * (PR_BM * 128) + (box << c.page_shift) * 128, tm, &full[stage], ch * 64, 0, it.head, page);
+            tma_load_4d(ring + pos.stage * Cfg::TILE_BYTES + ch * (PR_BM * 128) + (box << c.page_shift) * 128, tm, &full[pos.stage], ch * 64, 0, it.head,
+                        page);
           __syncwarp();
-          if (++stage == Cfg::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          pos.next();
           return true;
         };
         if (hi - it.lo <= 2) steal();
@@ -299,11 +318,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               ahead = hold(held_from + 32);
             }
             if (first_q) ok = load_q(0);
-            ok = ok && load_kv(&tmK, j);
+            ok = ok && load_kv(&tmK, sK, k_full, k_empty, k_at, j);
             if (second_q) ok = ok && load_q(1);
-            ok = ok && load_kv(&tmV, j);
+            ok = ok && load_kv(&tmV, sV, v_full, v_empty, v_at, j);
             first_q = second_q = false;
           }
+        }
+        // rows outside every sequence give zeros: an equal share with every index of the grid, items or not
+        for (long long z = (long long)idx * 32 + lane; z < outside; z += (long long)gridDim.x * 32) {
+          const long long r = z / row_vecs, row = r < begin ? r : end + (r - begin);
+          reinterpret_cast<uint4*>(p.out)[row * row_vecs + z % row_vecs] = make_uint4(0, 0, 0, 0);
         }
         ok = ok && mbar_wait(stolen, steal_phase, abort_flag, c.status, kStatusTimeoutFull);
         steal_phase ^= 1;
@@ -321,13 +345,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       constexpr uint32_t kLoK = (16u >> 4) << 16;                                       // K-major: LBO 16
       constexpr uint32_t kLoMN = ((uint32_t)(PR_BM * 128) >> 4) << 16;                  // MN-major V: 64-column chunks 16 KB apart
       auto desc = [&](uint32_t lo) -> uint64_t { return (static_cast<uint64_t>(kDescHi) << 32) | lo; };
-      const uint32_t q16 = (smem_u32(smem) & 0x3FFFF) >> 4, ring16 = (smem_u32(sRing) & 0x3FFFF) >> 4;
-      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, clean_phase = 0;
-      int stage = 0;
-      uint32_t phase = 0;
+      const uint32_t q16 = (smem_u32(smem) & 0x3FFFF) >> 4, k16 = (smem_u32(sK) & 0x3FFFF) >> 4, v16 = (smem_u32(sV) & 0x3FFFF) >> 4;
+      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      PrRing<Cfg::K_STAGES> k_at;
+      PrRing<Cfg::V_STAGES> v_at;
       bool ok = true;
       auto scores = [&](int w, int k_stage) {   // S_w = Q_w K^T
-        const uint32_t a = q16 + w * (Cfg::TILE_BYTES >> 4), bk = ring16 + k_stage * (Cfg::TILE_BYTES >> 4);
+        const uint32_t a = q16 + w * (Cfg::TILE_BYTES >> 4), bk = k16 + k_stage * (Cfg::TILE_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (PR_BM * 128 >> 4) + (kk & 3) * 2;
@@ -336,21 +360,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         if (leader) umma_commit(&s_full[w]);
         __syncwarp();
       };
-      auto take = [&](int& my_stage) -> bool {   // next tile of the ring
-        if (!mbar_wait(&full[stage], phase, abort_flag, c.status, kStatusTimeoutFull)) return false;
-        my_stage = stage;
-        if (++stage == Cfg::STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
+      auto take = [&](uint64_t* full, auto& pos, int& my_stage) -> bool {   // next tile of a ring
+        if (!mbar_wait(&full[pos.stage], pos.phase, abort_flag, c.status, kStatusTimeoutFull)) return false;
+        my_stage = pos.stage;
+        pos.next();
         return true;
+      };
+      auto take_v = [&](int& my_stage) -> bool {   // landed and looked over
+        return mbar_wait(&clean[v_at.stage], v_at.phase, abort_flag, c.status, kStatusTimeoutFull) && take(v_full, v_at, my_stage);
       };
       PrItem it;
       for (int i = 0; ok && take_item(i, it); ++i) {
         const int lo = it.lo, hi = max(it.hi[0], it.hi[1]);
         if (hi > lo) {
           int k_stage = 0, v_stage = 0;
-          ok = take(k_stage);
+          ok = take(k_full, k_at, k_stage);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             if (!ok || it.hi[w] <= lo) continue;
@@ -361,19 +385,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             scores(w, k_stage);
             if (leader && it.hi[w] == lo + 1) umma_commit(&q_empty[w]);
           }
-          if (ok && leader) umma_commit(&empty[k_stage]);
+          if (ok && leader) umma_commit(&k_empty[k_stage]);
           for (int j = lo; j < hi && ok; ++j) {
-            ok = take(v_stage);
-            if (ok) {
-              ok = mbar_wait(&clean[v_stage], (clean_phase >> v_stage) & 1, abort_flag, c.status, kStatusTimeoutFull);
-              clean_phase ^= 1u << v_stage;
-            }
-            if (ok && j + 1 < hi) ok = take(k_stage);
+            ok = take_v(v_stage);
+            if (ok && j + 1 < hi) ok = take(k_full, k_at, k_stage);
             if (!ok) break;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               if (!ok || j >= it.hi[w]) continue;
-              const uint32_t bv = ring16 + v_stage * (Cfg::TILE_BYTES >> 4);
+              const uint32_t bv = v16 + v_stage * (Cfg::TILE_BYTES >> 4);
               // O_w += P_w V: 16 keys per product, P_w from tensor memory, the first products before all of P_w is there
               ok = mbar_wait(&p_part[w], p_phase[w], abort_flag, c.status, kStatusTimeoutTmemFull);
               if (!ok) continue;
@@ -399,8 +419,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               __syncwarp();
             }
             if (ok && leader) {
-              umma_commit(&empty[v_stage]);
-              if (j + 1 < hi) umma_commit(&empty[k_stage]);
+              umma_commit(&v_empty[v_stage]);
+              if (j + 1 < hi) umma_commit(&k_empty[k_stage]);
             }
             __syncwarp();
           }
@@ -410,42 +430,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     } else {
       // ---------------------------------------------------------------- V tiles with late keys: 64 threads, two rows each
       const int tid = (warp - 2) * 32 + lane;
-      int stage = 0;   // ring position of the item's next K tile
-      uint32_t phase = 0;
+      PrRing<Cfg::V_STAGES> v_at;
       bool ok = true;
       PrItem it;
-      // rows outside every sequence give zeros
-      {
-        const int begin = min(max(c.offsets[0], 0), c.rows), end = min(max(c.offsets[c.seqs], begin), c.rows);
-        const long long row_vecs = (long long)c.Hq * (D / 8), outside = (long long)(begin + c.rows - end) * row_vecs;
-        for (long long i = (long long)blockIdx.x * 64 + tid; i < outside; i += (long long)gridDim.x * 64) {
-          const long long r = i / row_vecs, row = r < begin ? r : end + (r - begin);
-          reinterpret_cast<uint4*>(p.out)[row * row_vecs + i % row_vecs] = make_uint4(0, 0, 0, 0);
-        }
-      }
       for (int i = 0; ok && take_item(i, it); ++i) {
         const int hi = max(it.hi[0], it.hi[1]), late = late_from(it);
         for (int j = it.lo; j < hi && ok; ++j) {
-          int v_stage = stage + 1;
-          uint32_t v_phase = phase;
-          if (v_stage == Cfg::STAGES) {
-            v_stage = 0;
-            v_phase ^= 1;
-          }
-          stage = v_stage + 1;
-          phase = v_phase;
-          if (stage == Cfg::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
-          // every V tile passes through here, so that these warps keep step with the ring
-          ok = mbar_wait(&full[v_stage], v_phase, abort_flag, c.status, kStatusTimeoutFull);
+          const int v_stage = v_at.stage;
+          ok = mbar_wait(&v_full[v_stage], v_at.phase, abort_flag, c.status, kStatusTimeoutFull);
           if (!ok) break;
+          v_at.next();
           if ((j + 1) * PR_BM <= late) {
             if (lane == 0) mbar_arrive(&clean[v_stage]);
             continue;
           }
-          uint8_t* tile = sRing + v_stage * Cfg::TILE_BYTES;
+          uint8_t* tile = sV + v_stage * Cfg::TILE_BYTES;
 #pragma unroll 1
           for (int row = tid; row < PR_BM; row += 64) {
             const int key = j * PR_BM + row;
@@ -665,13 +664,22 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
   float sum = weight * ml.y, acc[PER] = {};
 #pragma unroll
   for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-#pragma unroll 4
-  for (int i = 0; i < p.splits; ++i) {
-    const float f = __shfl_sync(0xffffffffu, weight, i);
-    if (f == 0.f) continue;
-    const float* src = p.part_o + (i * n + at) * D + lane * PER;
+  for (int i0 = 0; i0 < p.splits; i0 += 8) {   // eight parts on their way at a time
+    float part[8][PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] += f * src[e];
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u < p.splits) {
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(&part[u][e]) = *reinterpret_cast<const float2*>(p.part_o + ((i0 + u) * n + at) * D + lane * PER + e);
+      }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float f = __shfl_sync(0xffffffffu, weight, (i0 + u) & 31);
+      if (i0 + u < p.splits && f != 0.f) {   // a part without weight was not written
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] += f * part[u][e];
+      }
+    }
   }
   const float inv = nowhere ? 0.f : 1.f / sum;
 #pragma unroll
@@ -683,23 +691,26 @@ struct PrPlan {
   long long items, bytes;
 };
 
+// Query tiles of an item and CTAs that share its keys, by the time that the longest items take in all, in ns.  Measured at
+// head_dim 128 (24 / 8 heads) and 64 (32 / 4): a K / V tile takes a pair of query tiles 1580 and a single one 1460, an item's
+// beginning and end 1500, the joining kernel 3500 and its parts' bytes.  256 tokens behind 32768: single tiles and two splits
+// 214 us, pairs and four 130 us; 500 tokens alone: single tiles 14.1 us, pairs 15.0, two splits 25.8.
 static PrPlan pr_plan(const incin_paged_desc* d) {
-  PrPlan pl;
+  PrPlan pl = {};
   const int sms = device_sm_count();
   pl.tokens = PR_BM / (d->Hq / d->Hkv);
-  auto items = [&](int tiles) { return ((long long)d->rows / (tiles * pl.tokens) + d->seqs) * d->Hkv; };   // at most
-  pl.tiles = 2;
-  pl.splits = 1;
-  if (items(1) <= sms) pl.tiles = 1;
-  // keys of a sequence at most, in tiles
-  const long long keys = ((long long)d->table_width * d->page_size + PR_BM - 1) / PR_BM;
-  const long long n = ((long long)d->rows + pl.tiles * pl.tokens - 1) / (pl.tiles * pl.tokens) * d->Hkv;
-  if (n * 2 <= sms) {
-    long long s = sms / n;
-    if (s > keys / 4) s = keys / 4;
-    pl.splits = s < 1 ? 1 : s > 32 ? 32 : (int)s;
-  }
-  pl.items = items(pl.tiles) * pl.splits;
+  const long long keys = ((long long)d->table_width * d->page_size + PR_BM - 1) / PR_BM;   // K / V tiles of a sequence at most
+  double best = 0;
+  for (int tiles = 1; tiles <= 2; ++tiles)
+    for (int splits = 1; splits <= 32 && (splits == 1 || splits * 2 <= keys); ++splits) {
+      const long long n = (((long long)d->rows + tiles * pl.tokens - 1) / (tiles * pl.tokens) + (d->seqs - 1) / 2) * d->Hkv * splits;
+      if (splits > 1 && n > 2 * sms) break;
+      const double rounds = n <= 3 * sms ? (double)((n + sms - 1) / sms) : (double)n / sms + 0.5;
+      double time = rounds * ((double)((keys + splits - 1) / splits) * (tiles == 2 ? 1580 : 1460) + 1500);
+      if (splits > 1) time += 3500 + (double)splits * d->rows * d->Hq * d->D * 8 / 4000;
+      if (pl.tiles == 0 || time < best) best = time, pl.tiles = tiles, pl.splits = splits;
+    }
+  pl.items = ((long long)d->rows / (pl.tiles * pl.tokens) + d->seqs) * d->Hkv * pl.splits;   // at most
   pl.bytes = pl.splits > 1 ? (long long)pl.splits * d->rows * d->Hq * (d->D * 4 + 8) : 0;
   return pl;
 }

@@ -237,6 +237,38 @@ def test_prompt_later_tokens_stay_out(hq, hkv, D, at):
     assert torch.isfinite(out[300:]).all()
 
 
+@pytest.mark.parametrize("new,pad", [([1], 6000), ([700, 3], 4000), ([0, 0], 900), ([2000] * 3, 5000)])
+def test_prompt_padded_batch(new, pad):
+    """Many rows behind the last sequence, more than the work of the real ones: all of them zeros."""
+    hq, hkv, D = 32, 4, 64
+    k, v, table, lens = make_cache([max(n, 1) for n in new], hkv, 64, D, torch.bfloat16, "cuda")
+    offsets = _i32(0, *torch.tensor(new).cumsum(0).tolist())
+    q = _randn(sum(new) + pad, hq, D, dtype=torch.bfloat16, seed=9)
+    for _ in range(5):
+        torch.empty(q.shape, dtype=q.dtype, device="cuda").fill_(float("nan"))    # what the output's memory held before
+        out = _F().prompt_attention(q, k, v, table, lens, offsets)
+        assert not out[sum(new):].any()
+    _check_attention(q, k, v, table, lens, offsets)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(24, 8, 128), (32, 4, 64)])
+@pytest.mark.parametrize("new,past", [([4], [32000]), ([100], [16000]), ([700, 900], [3000, 0])])
+def test_prompt_repeats_to_the_bit(hq, hkv, D, new, past):
+    """Calls in a row without waiting, over a cache larger than L2 among others: K and V tiles land out of order, calls overlap
+    at their ends.  Sums have a fixed order, so any product that starts before its operands are complete shows up."""
+    lengths = [a + b for a, b in zip(new, past)]
+    offsets = _i32(0, *torch.tensor(new).cumsum(0).tolist())
+    q = _randn(sum(new), hq, D, dtype=torch.bfloat16, seed=10)
+    caches = [make_cache(lengths, hkv, 64, D, torch.bfloat16, "cuda", seed=s) for s in range(3)]
+    first = [_F().prompt_attention(q, *c, offsets) for c in caches]
+    _status()
+    for _ in range(20):
+        outs = [_F().prompt_attention(q, *c, offsets) for c in caches]
+        for a, b in zip(outs, first):
+            assert _same(a, b)
+    _status()
+
+
 def test_strided_queries_and_other_scales():
     hq, hkv, D = 8, 2, 64
     k, v, table, lens = make_cache([90, 40, 17], hkv, 32, D, torch.float16, "cuda")
