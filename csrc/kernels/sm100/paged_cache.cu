@@ -131,10 +131,14 @@ extern "C" int incin_kv_append(const incin_paged_desc* d, double theta, void* st
   const int rc = check_paged(d);
   if (rc) return rc;
   if (!(theta == 0.0 || (theta >= 1.0 && theta < 1e300)) || (!d->offsets && d->rows != d->seqs)) return INCIN_ERR_ARGUMENT;
-  RopeTurns turns = {};
-  if (theta != 0.0)
+  static thread_local RopeTurns turns;   // of the last theta and head_dim: a model's layers share them
+  static thread_local double of_theta = 0.0;
+  static thread_local int of_dim = 0;
+  if (theta != 0.0 && (theta != of_theta || d->D != of_dim)) {
     for (int i = 0; i < d->D / 2; ++i)   // at most 1 / (2 pi) of a turn
       turns.per_token[i] = (uint64_t)std::ldexp(std::pow(theta, -2.0 * i / d->D) / 6.283185307179586476925, 64);
+    of_theta = theta, of_dim = d->D;
+  }
   const cudaStream_t s = (cudaStream_t)stream;
   const int rotate = theta != 0.0;
   const bool half = d->dtype == INCIN_GEMM_IN_FP16;

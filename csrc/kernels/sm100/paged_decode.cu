@@ -44,7 +44,7 @@ struct DecParams {
   float scale_log2;
   int unit;            // tokens of a unit of work, a multiple of DEC_STEP
   int group, chunks;   // query heads of a key head, and the blocks of HEADS they are dealt in
-  int4* open;          // per CTA: {sequence, head block, last CTA} of the pair that it begins and others continue, or -1
+  int4* open;          // per CTA: {sequence, head block, last CTA} of the pair that it begins and others continue, or -1; NULL where none can
   float* parts;        // per CTA two slots: the continuation of a pair, the beginning of one
 };
 
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   const long long units = (long long)before[c.seqs] * head_blocks;
   const int ctas = (int)min((long long)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) {
-    if (threadIdx.x == 0) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
   long long u = dec_start(units, blockIdx.x, ctas);
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     if (u >= u_end) break;
     __syncthreads();
   }
-  if (threadIdx.x == 0) p.open[blockIdx.x] = opened;
+  if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = opened;
 }
 
 // Block (i, y): joins the parts of the pair that CTA i began, if it began one, for the query heads [y HB, (y + 1) HB).  A head
@@ -475,7 +475,7 @@ static DecPlan dec_plan(const incin_paged_desc* d) {
   const long long room = (long long)device_sm_count() * Cfg::CTAS_PER_SM;
   pl.grid = (int)(most < room ? most : room);
   pl.splits = per_pair > 1;
-  pl.bytes = (long long)pl.grid * (16 + 2 * Cfg::SLOT * 4);
+  pl.bytes = pl.splits ? (long long)pl.grid * (16 + 2 * Cfg::SLOT * 4) : 0;
   return pl;
 }
 
@@ -483,9 +483,10 @@ template <typename T, int D, int NT>
 static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
   using Cfg = DecCfg<D, NT>;
   const DecPlan pl = dec_plan<D, NT>(d);
+  if (pl.splits && !d->workspace) return INCIN_ERR_ARGUMENT;
   if ((long long)d->table_width * d->page_size > (1ll << 37) / DEC_SEQS) return INCIN_ERR_TOO_LARGE;   // units are counted in 32 bits
   DecParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
-                 pl.unit, d->Hq / d->Hkv, pl.chunks, (int4*)d->workspace, (float*)((char*)d->workspace + 16ll * pl.grid)};
+                 pl.unit, d->Hq / d->Hkv, pl.chunks, pl.splits ? (int4*)d->workspace : nullptr, (float*)((char*)d->workspace + 16ll * pl.grid)};
   p.c.offsets = nullptr;
   static PerDeviceFlags main_set, join_set, wide_join_set;
   if (!shared_split(decode_attention_kernel<T, D, NT>, Cfg::SHARED, main_set) || !shared_split(decode_join_kernel<T, D, NT, 1>, Cfg::SHARED, join_set) ||
@@ -525,7 +526,7 @@ extern "C" int incin_decode_attention(const incin_paged_desc* d, void* stream) {
   using namespace incin;
   const int rc = check_paged(d);
   if (rc) return rc;
-  if (d->rows != d->seqs || !d->workspace) return INCIN_ERR_ARGUMENT;
+  if (d->rows != d->seqs) return INCIN_ERR_ARGUMENT;
   const cudaStream_t s = (cudaStream_t)stream;
   const bool one = d->Hq / d->Hkv <= 8;
   auto run = [&](auto t) {

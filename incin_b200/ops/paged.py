@@ -55,70 +55,78 @@ _KIND = {torch.bfloat16: nat.GEMM_IN_BF16, torch.float16: nat.GEMM_IN_FP16}
 
 
 # ------------------------------------------------------------------------------------------------------------- checks
-def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int) -> None:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int):
+    """The strides of the pages, once everything about the arguments is in order (these checks and the descriptor are most
+    of a short call's time: no attribute is asked for twice)."""
+    shape, dtype, device = k_pages.shape, x.dtype, x.device
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages must both be [pages, kv_heads, page_size, head_dim], got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    pages, hkv, size, D = k_pages.shape
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    pages, hkv, size, D = shape
     if size not in PAGE_SIZES:
         raise ValueError(f"{what}: page_size must be one of {PAGE_SIZES}, got {size}")
-    if not (x.dtype == k_pages.dtype == v_pages.dtype and x.dtype.is_floating_point):
-        raise ValueError(f"{what}: rows and pages must have one float type, got {x.dtype}, {k_pages.dtype} and {v_pages.dtype}")
+    if dtype is not k_pages.dtype or dtype is not v_pages.dtype or not dtype.is_floating_point:
+        raise ValueError(f"{what}: rows and pages must have one float type, got {dtype}, {k_pages.dtype} and {v_pages.dtype}")
     if pages == 0 or hkv == 0 or n_heads <= 0 or n_heads % hkv:
         raise ValueError(f"{what}: {n_heads} query heads do not fall into {hkv} key heads ({pages} pages)")
-    if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != lengths.shape[0] or table.shape[0] == 0 or table.shape[1] == 0:
-        raise ValueError(f"{what}: table must be [sequences, entries] and lengths [sequences], got {tuple(table.shape)} and "
-                         f"{tuple(lengths.shape)}")
-    seqs = table.shape[0]
+    t_shape, l_shape = table.shape, lengths.shape
+    if len(t_shape) != 2 or len(l_shape) != 1 or t_shape[0] != l_shape[0] or t_shape[0] == 0 or t_shape[1] == 0:
+        raise ValueError(f"{what}: table must be [sequences, entries] and lengths [sequences], got {tuple(t_shape)} and "
+                         f"{tuple(l_shape)}")
+    seqs = t_shape[0]
     if offsets is None:
         if rows != seqs:
             raise ValueError(f"{what}: {rows} rows for {seqs} sequences (one row each, or offsets)")
-    elif offsets.dim() != 1 or offsets.shape[0] != seqs + 1:
+    elif tuple(offsets.shape) != (seqs + 1,):
         raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
     for name, t in (("table", table), ("lengths", lengths), ("offsets", offsets)):
-        if t is not None and (t.dtype != torch.int32 or t.stride(-1) != 1):
+        if t is not None and (t.dtype is not torch.int32 or t.stride(-1) != 1):
             raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
     for t in (k_pages, v_pages, table, lengths, offsets):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
-    if x.is_cuda:
-        if x.dtype not in _KIND or D not in (64, 128):
-            raise nat.NativeError(f"{what}: no kernel for {x.dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
-        if n_heads // hkv > 128:
-            raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
-        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
-                raise nat.NativeError(f"{what}: {name} needs contiguous rows that start on 16-byte boundaries, got strides {t.stride()}")
+    if device.type != "cuda":
+        return None
+    if dtype not in _KIND or D not in (64, 128):
+        raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
+    if n_heads // hkv > 128:
+        raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
+    return _page_strides(what, "k_pages", k_pages) + _page_strides(what, "v_pages", v_pages)
+
+
+def _page_strides(what: str, name: str, t) -> tuple[int, int, int]:
+    a, b, c, d = t.stride()
+    if d != 1 or a % 8 or b % 8 or c % 8 or min(a, b, c) <= 0 or t.data_ptr() % 16:
+        raise nat.NativeError(f"{what}: {name} needs contiguous rows that start on 16-byte boundaries, got strides {t.stride()}")
+    return a, b, c
 
 
 def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """``x`` with contiguous heads that start on 16-byte boundaries."""
-    if x.stride(-1) == 1 and not any(s % 8 for s in x.stride()[:-1]) and x.data_ptr() % 16 == 0:
+    """``x`` ``[rows, heads, head_dim]`` with contiguous heads that start on 16-byte boundaries, none of them shared."""
+    a, b, c = x.stride()
+    if c == 1 and a > 0 and b > 0 and not (a % 8 or b % 8 or x.data_ptr() % 16):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _launch(fn, what: str, x, k_pages, v_pages, table, lengths, offsets, n_heads: int, out, scale: float = 0.0, args=(), workspace=None):
+def _launch(fn, what: str, x, k_pages, v_pages, table, lengths, offsets, strides, out, scale: float = 0.0, args=(), workspace=None):
     pages, hkv, size, D = k_pages.shape
-    d = PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], *v_pages.stride()[:3], table.data_ptr(),
-                  table.stride(0), lengths.data_ptr(), nat.ptr(offsets), table.shape[1], table.shape[0], x.shape[0], pages, size,
-                  n_heads, hkv, D, _KIND[x.dtype], scale, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), None,
-                  status_word(x.device).data_ptr())
+    seqs, width = table.shape
+    x_row, x_head, _ = x.stride()
+    d = PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), *strides, table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                  None if offsets is None else offsets.data_ptr(), width, seqs, x.shape[0], pages, size, out.shape[1], hkv, D,
+                  _KIND[x.dtype], scale, x.data_ptr(), x_row, x_head, out.data_ptr(), None, status_word(x.device).data_ptr())
+    at = C.byref(d)
     room = None
     if workspace is not None:
-        n = workspace(C.byref(d))
+        n = workspace(at)
         if n:   # of this call alone: two captured graphs share none
             room = torch.empty(n, dtype=torch.uint8, device=x.device)
             d.workspace = room.data_ptr()
-    nat.check(fn(C.byref(d), *args, nat.stream_ptr()), what)
+    nat.check(fn(at, *args, nat.stream_ptr()), what)
     return out
-
-
-def _on(t: torch.Tensor):
-    """The device of ``t`` made current where it is another one."""
-    return torch.cuda.device(t.device)
 
 
 def _is_current(t: torch.Tensor) -> bool:
@@ -141,17 +149,17 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
         raise ValueError(f"kv_append: rows of {qkv.shape[1]} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
     if theta is not None and not 1.0 <= theta < 1e300:
         raise ValueError(f"kv_append: theta must be at least 1, got {theta}")
-    _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    strides = _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     x = qkv.unflatten(1, (n_heads + 2 * hkv, D))
     if not qkv.is_cuda:
         return _append_cpu(x, k_pages, v_pages, table, lengths, offsets, n_heads, theta)
     if not _is_current(qkv):
-        with _on(qkv):
+        with torch.cuda.device(qkv.device):
             return kv_append(qkv, k_pages, v_pages, table, lengths, offsets, n_heads=n_heads, theta=theta)
     q = torch.empty(rows, n_heads, D, dtype=qkv.dtype, device=qkv.device)
     if rows == 0:
         return q
-    return _launch(nat.cuda().incin_kv_append, "kv_append", _rows16(x), k_pages, v_pages, table, lengths, offsets, n_heads, q,
+    return _launch(nat.cuda().incin_kv_append, "kv_append", _rows16(x), k_pages, v_pages, table, lengths, offsets, strides, q,
                    args=(theta or 0.0,))
 
 
@@ -176,14 +184,14 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
         raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(q.shape)} and pages "
                          f"{tuple(k_pages.shape)}")
     rows, n_heads, D = q.shape
-    _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    strides = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale < 0:
         raise ValueError(f"{what}: scale must be finite and not negative, got {scale}")
     if not q.is_cuda:
         return _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale)
     if not _is_current(q):
-        with _on(q):
+        with torch.cuda.device(q.device):
             return _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale)
     out = torch.empty(rows, n_heads, D, dtype=q.dtype, device=q.device)
     if rows == 0:
@@ -191,7 +199,7 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
     lib = nat.cuda()
     fn, room = ((lib.incin_decode_attention, lib.incin_decode_attention_workspace) if offsets is None else
                 (lib.incin_prompt_attention, lib.incin_prompt_attention_workspace))
-    return _launch(fn, what, _rows16(q), k_pages, v_pages, table, lengths, offsets, n_heads, out, scale, workspace=room)
+    return _launch(fn, what, _rows16(q), k_pages, v_pages, table, lengths, offsets, strides, out, scale, workspace=room)
 
 
 # -------------------------------------------------------------------------------------------------------------- pages
@@ -232,7 +240,7 @@ def copy_pages(storage, src, dst):
     if storage.data_ptr() % 16:
         raise nat.NativeError("copy_pages: storage must start on a 16-byte boundary")
     if not _is_current(storage):
-        with _on(storage):
+        with torch.cuda.device(storage.device):
             return copy_pages(storage, src, dst)
     src, dst = src.contiguous(), dst.contiguous()
     nat.check(nat.cuda().incin_copy_pages(storage.data_ptr(), src.data_ptr(), dst.data_ptr(), src.numel(), outer, pages, page_bytes,
