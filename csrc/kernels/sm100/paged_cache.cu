@@ -14,29 +14,54 @@ struct RopeTurns {
   uint64_t per_token[64];   // theta^(-2i/D) / (2 pi), in units of 2^-64 turns
 };
 
-constexpr int APPEND_ROWS = 8;
+// A block takes up to eight rows.  A thread asks for its first 32 bytes before anything is known about their place: which
+// sequence, which position and page and the angles are a chain of four loads that the data need not wait for.  (More than
+// 32 bytes ahead cost occupancy: 8190 rows of 40 heads of 128, 33.2 us, 64 bytes 35.1, 128 bytes 36.6.)  Bound by memory.
+constexpr int APPEND_ROWS = 8, APPEND_BLOCK_BYTES = 40 << 10;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_append_kernel(const PagedView c, const uint16_t* x, long long x_row, long long x_head, uint16_t* q,
                                                         const __grid_constant__ RopeTurns turns, int rotate, int tokens) {
   constexpr int HALF = D / 2, VECS = HALF / 8;
   __shared__ float2 angle[APPEND_ROWS * HALF];
-  __shared__ int seq_of[APPEND_ROWS], pos_of[APPEND_ROWS], page_of[APPEND_ROWS];
+  __shared__ int pos_of[APPEND_ROWS], page_of[APPEND_ROWS];   // -1 where there is none
   pdl_launch_dependents();
   pdl_wait();
-  const int first = blockIdx.x * tokens, n = min(tokens, c.rows - first), heads = c.Hq + 2 * c.Hkv;
-  if (threadIdx.x < n) {
-    const int t = first + threadIdx.x, s = paged_sequence(c, t);
-    int pos = -1, page = -1;
+  const int first = blockIdx.x * tokens, n = min(tokens, c.rows - first), per = (c.Hq + 2 * c.Hkv) * VECS, total = n * per;
+  uint4 lo, hi;
+  auto load = [&](int i) {
+    if (i < total) {
+      const int r = i / per, k = i - r * per;
+      const uint16_t* src = x + (first + r) * x_row + k / VECS * x_head + k % VECS * 8;
+      lo = *reinterpret_cast<const uint4*>(src);
+      hi = *reinterpret_cast<const uint4*>(src + HALF);
+    }
+  };
+  load(threadIdx.x);
+  if (threadIdx.x < 32) {
+    const int t = first + threadIdx.x;
+    int s = -1, pos = -1, page = -1;
+    if (!c.offsets) {
+      if (threadIdx.x < n && t < c.seqs) s = t;
+    } else {   // sequences that end in front of the block's first row; a row's own lies there or a little behind
+      int ended = 0;
+      for (int i = threadIdx.x; i - (int)threadIdx.x < c.seqs; i += 32) ended += __popc(__ballot_sync(0xffffffffu, i < c.seqs && c.offsets[i + 1] <= first));
+      if (threadIdx.x < n) {
+        s = ended;
+        while (s < c.seqs && c.offsets[s + 1] <= t) ++s;
+        if (s >= c.seqs || c.offsets[s] > t) s = -1;
+      }
+    }
     if (s >= 0) {
       const int len = paged_length(c, s);
       pos = c.offsets ? len - c.offsets[s + 1] + t : len - 1;
       if (pos >= 0) page = paged_page(c, s, pos >> c.page_shift);
       else if (c.offsets) flag_bad_index(c.status);   // more new rows than tokens; without offsets an idle sequence
     }
-    seq_of[threadIdx.x] = pos >= 0 ? s : -1;
-    pos_of[threadIdx.x] = pos;
-    page_of[threadIdx.x] = page;
+    if (threadIdx.x < n) {
+      pos_of[threadIdx.x] = pos;
+      page_of[threadIdx.x] = page;
+    }
   }
   __syncthreads();
   if (rotate) {
@@ -48,25 +73,21 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const PagedView c, const
     }
     __syncthreads();
   }
-  const int per = heads * VECS;
-  for (int i = threadIdx.x; i < n * per; i += 256) {
-    const int r = i / per, k = i - r * per, h = k / VECS, v = (k - h * VECS) * 8;
+  for (int i = threadIdx.x; i < total; i += 256) {
+    if (i >= 256) load(i);
+    const int r = i / per, k = i - r * per, h = k / VECS, v = k % VECS * 8, pos = pos_of[r];
     uint16_t* dst;
     if (h < c.Hq) {
       dst = q + ((long long)(first + r) * c.Hq + h) * D;
-      if (seq_of[r] < 0) {
-        *reinterpret_cast<uint4*>(dst + v) = *reinterpret_cast<uint4*>(dst + HALF + v) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
+      if (pos < 0) lo = hi = make_uint4(0, 0, 0, 0);
     } else {
-      if (page_of[r] < 0) continue;
-      const int slot = pos_of[r] & ((1 << c.page_shift) - 1), hk = h - c.Hq;
-      dst = hk < c.Hkv ? const_cast<uint16_t*>(c.k) + page_of[r] * c.k_page + hk * c.k_head + slot * c.k_token
-                       : const_cast<uint16_t*>(c.v) + page_of[r] * c.v_page + (hk - c.Hkv) * c.v_head + slot * c.v_token;
+      const int page = page_of[r];
+      if (page < 0) continue;
+      const int slot = pos & ((1 << c.page_shift) - 1), hk = h - c.Hq;
+      dst = hk < c.Hkv ? const_cast<uint16_t*>(c.k) + page * c.k_page + hk * c.k_head + slot * c.k_token
+                       : const_cast<uint16_t*>(c.v) + page * c.v_page + (hk - c.Hkv) * c.v_head + slot * c.v_token;
     }
-    const uint16_t* src = x + (first + r) * x_row + h * x_head;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + v), hi = *reinterpret_cast<const uint4*>(src + HALF + v);
-    if (rotate && h < c.Hq + c.Hkv) {
+    if (rotate && h < c.Hq + c.Hkv && pos >= 0) {
       uint32_t *a = &lo.x, *b = &hi.x;
       const float2* cs = angle + r * HALF + v;
 #pragma unroll
@@ -118,8 +139,11 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(uint4* storage
 
 template <typename T, int D>
 static cudaError_t launch_append(const incin_paged_desc* d, const RopeTurns& turns, int rotate, cudaStream_t stream) {
+  // rows of about 40 KB a block: 8190 rows of 40 heads of 128, 8 a block 34.1 us, 4 33.2; 8000 of 40 heads of 64, 8 17.1, 4 17.9, 2
+  // 19.2; but at least two blocks an SM
+  const long long row_bytes = (d->Hq + 2ll * d->Hkv) * D * 2;
   int tokens = APPEND_ROWS;
-  while (tokens > 1 && d->rows < 2 * device_sm_count() * tokens) tokens /= 2;
+  while (tokens > 1 && (d->rows < 2 * device_sm_count() * tokens || tokens * row_bytes > APPEND_BLOCK_BYTES * 5 / 4)) tokens /= 2;
   return launch_pdl(kv_append_kernel<T, D>, dim3((d->rows + tokens - 1) / tokens), dim3(256), 0, stream, paged_view(d), (const uint16_t*)d->x,
                     d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, turns, rotate, tokens);
 }
