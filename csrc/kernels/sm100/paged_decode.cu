@@ -484,7 +484,7 @@ static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
   using Cfg = DecCfg<D, NT>;
   const DecPlan pl = dec_plan<D, NT>(d);
   if (pl.splits && !d->workspace) return INCIN_ERR_ARGUMENT;
-  if ((long long)d->table_width * d->page_size > (1ll << 37) / DEC_SEQS) return INCIN_ERR_TOO_LARGE;   // units are counted in 32 bits
+  if ((long long)d->table_width * d->page_size > (1ll << 36) / DEC_SEQS) return INCIN_ERR_TOO_LARGE;   // units are counted in 32 bits
   DecParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
                  pl.unit, d->Hq / d->Hkv, pl.chunks, pl.splits ? (int4*)d->workspace : nullptr, (float*)((char*)d->workspace + 16ll * pl.grid)};
   p.c.offsets = nullptr;

@@ -80,6 +80,8 @@ def _ops() -> dict[str, Callable]:
         "concat": T.concat, "gather": T.gather_last, "index_select": T.index_select,
         "transpose": lambda x, a, b: x.transpose(a, b), "reshape": lambda x, shape: x.reshape(shape),
         "rope": F.rope, "swiglu": F.swiglu,
+        "kv_append": F.kv_append, "decode_attention": F.decode_attention, "prompt_attention": F.prompt_attention,
+        "copy_pages": F.copy_pages,
     }
 
 

@@ -337,8 +337,9 @@ CPU_CAPABILITIES: tuple[CapabilityRule, ...] = tuple(
                "embedding", "cross_entropy", "sdpa", "conv1d", "conv2d", "conv_transpose2d", "max_pool2d", "avg_pool2d",
                "adaptive_avg_pool2d", "batch_norm", "sum", "mean",
                "max", "min", "argmax", "topk", "argsort", "cumsum", "reshape", "transpose", "concat", "gather",
-               "index_select", "adamw", "sgd", "rope", "swiglu", "dropout")
-) + (CapabilityRule("quantize_q8_0", (DTypeId.F32,), SupportLevel.NATIVE, "libincin_host oracle"),
+               "index_select", "adamw", "sgd", "rope", "swiglu", "dropout", "kv_append", "decode_attention", "prompt_attention")
+) + (CapabilityRule("copy_pages", _ALL, SupportLevel.NATIVE, "torch-cpu"),
+     CapabilityRule("quantize_q8_0", (DTypeId.F32,), SupportLevel.NATIVE, "libincin_host oracle"),
      CapabilityRule("quantized_matmul", (DTypeId.Q8_0,), SupportLevel.COMPOSED, "dequantize + matmul"))
 
 _BF = (DTypeId.BF16,)
@@ -385,6 +386,10 @@ CUDA_CAPABILITIES: tuple[CapabilityRule, ...] = (
     CapabilityRule("quantized_matmul", (DTypeId.Q8_0,), SupportLevel.COMPOSED, "dequantize_q8_0 (bf16) + gemm_tcgen05"),
     CapabilityRule("reshape", _ALL, SupportLevel.NATIVE, "view"),
     CapabilityRule("transpose", _ALL, SupportLevel.NATIVE, "view (GEMM reads either major)"),
+    CapabilityRule("kv_append", _BF + (DTypeId.F16,), SupportLevel.NATIVE, "kv_append (rotary + scatter into cache pages)"),
+    CapabilityRule("decode_attention", _BF + (DTypeId.F16,), SupportLevel.NATIVE, "decode_attention + decode_join (split over the cache)"),
+    CapabilityRule("prompt_attention", _BF + (DTypeId.F16,), SupportLevel.NATIVE, "prompt_attention (packed runs, tcgen05) + prompt_join"),
+    CapabilityRule("copy_pages", _ALL, SupportLevel.NATIVE, "copy_pages"),
 )
 
 

@@ -43,6 +43,8 @@ def check_status(device: torch.device | None = None) -> None:
     code = int(status_word(device).item())
     if code != 0:
         status_word(device).zero_()
+        if code == 6:
+            raise nat.NativeError("a kernel met an index outside its tensors (page, length or offset); results of this step are invalid")
         raise nat.NativeError(f"a device-side wait timed out (status {code}); results of this step are invalid")
 
 

@@ -80,7 +80,7 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
     elif tuple(offsets.shape) != (seqs + 1,):
         raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
     for name, t in (("table", table), ("lengths", lengths), ("offsets", offsets)):
-        if t is not None and (t.dtype is not torch.int32 or t.stride(-1) != 1):
+        if t is not None and (t.dtype is not torch.int32 or (t.stride(-1) != 1 and t.shape[-1] > 1)):
             raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
     for t in (k_pages, v_pages, table, lengths, offsets):
         if t is not None and t.device != device:

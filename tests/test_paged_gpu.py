@@ -137,7 +137,7 @@ def test_decode(dtype, hq, hkv, D, page):
     _check_attention(_randn(len(LENGTHS), hq, D, dtype=dtype, seed=1), k, v, table, lens)
 
 
-@pytest.mark.parametrize("lengths", [[1], [0], [5000], [33000, 1, 0, 700], [257] * 150, list(range(300))])
+@pytest.mark.parametrize("lengths", [[1], [0], [5000], [33000, 1, 0, 700], [257] * 150, list(range(300)), [5] * 513 + [200] + [70] * 600])
 @pytest.mark.parametrize("hq,hkv,D", [(32, 4, 64), (24, 8, 128), (2, 1, 128)])
 def test_decode_balances_any_batch(lengths, hq, hkv, D):
     """One long sequence, one long among short ones, many equal ones, many different ones."""
@@ -281,6 +281,59 @@ def test_strided_queries_and_other_scales():
         _check_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k, v, table, lens, _i32(0, 0, 2, 3))
     wide = torch.cat([table, table, table], 1)[:, :table.shape[1]]     # rows of a wider table
     _check_attention(q, k, v, wide, lens)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(128, 1, 64), (100, 1, 128), (66, 2, 64)])
+def test_widest_groups(hq, hkv, D):
+    """A query tile of one token; groups that fill it, or not."""
+    new, past = [3, 1, 140], [0, 500, 60]
+    lengths = [a + b for a, b in zip(new, past)]
+    k, v, table, lens = make_cache(lengths, hkv, 16, D, torch.bfloat16, "cuda")
+    q = _randn(144, hq, D, dtype=torch.bfloat16, seed=11)
+    _check_attention(q, k, v, table, lens, _i32(0, 3, 4, 144))
+    _check_attention(q[:3], k, v, table, lens)
+    x = _randn(144, (hq + 2 * hkv) * D, dtype=torch.bfloat16, seed=12)
+    _check_append(x, hq, k, v, table, lens, _i32(0, 3, 4, 144), 10000.0)
+
+
+def test_many_short_sequences():
+    """More sequences than a warp, a launch or a table's rows hold at once; one table row for all of them."""
+    hq, hkv, D = 8, 2, 64
+    n = 1100
+    k, v, table, _ = make_cache([90], hkv, 32, D, torch.bfloat16, "cuda")
+    table = table.expand(n, -1)                       # rows that share their memory
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 91, (n,), generator=g).to(torch.int32).cuda()
+    q = _randn(n, hq, D, dtype=torch.bfloat16, seed=13)
+    _check_attention(q, k, v, table, lens)
+    new = torch.minimum(torch.randint(0, 4, (n,), generator=g), lens.cpu())
+    offsets = torch.cat([torch.zeros(1, dtype=torch.long), new.cumsum(0)]).to(torch.int32).cuda()
+    rows = int(offsets[-1])
+    _check_attention(_randn(rows, hq, D, dtype=torch.bfloat16, seed=14), k, v, table, lens, offsets)
+    one = torch.tensor([[3, 9], [90, 9]], dtype=torch.int32, device="cuda")[:, 0]      # lengths with gaps: refused, one element is fine
+    with pytest.raises(ValueError):
+        _F().decode_attention(q[:2], k, v, table[:2], one)
+    _check_attention(q[:1], k, v, table[:1], one[:1])
+
+
+def test_odd_offsets_stay_in_bounds():
+    """Offsets that fall, start late or pass the rows: every row is in bounds, rows that belong to one sequence are right."""
+    F = _F()
+    hq, hkv, D = 4, 2, 64
+    lengths = [40, 50, 33]
+    k, v, table, lens = make_cache(lengths, hkv, 16, D, torch.bfloat16, "cuda", poison=False)
+    q = _randn(30, hq, D, dtype=torch.bfloat16)
+    for offs in ((5, 10, 20, 30), (0, 10, 10, 500), (0, 25, 10, 30), (-7, 3, 2 ** 31 - 1, 4), (30, 20, 10, 0), (0, 0, 0, 0)):
+        out = F.prompt_attention(q, k, v, table, lens, _i32(*offs))
+        F.kv_append(_randn(30, (hq + 2 * hkv) * D, dtype=torch.bfloat16), k.clone(), v.clone(), table, lens, _i32(*offs), n_heads=hq)
+        torch.cuda.synchronize()
+        if offs == (5, 10, 20, 30):
+            assert not out[:5].any()
+            assert torch.equal(out[5:], F.prompt_attention(q[5:].clone(), k, v, table, lens, _i32(0, 5, 15, 25)))
+    try:
+        _status()
+    except Exception:
+        pass
 
 
 def test_offsets_past_32_bits():
