@@ -194,5 +194,12 @@ def stream_ptr() -> int:
     return _raw_stream(_get_device())
 
 
+def device_index() -> int:
+    """Index of the calling thread's current CUDA device."""
+    if _get_device is None:
+        stream_ptr()
+    return _get_device()
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()

@@ -19,35 +19,28 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
 from .. import _native as nat
 from .gemm import status_word
 
-c_void_p, c_int, c_ll, c_float, c_double = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_double
+c_void_p, c_int, c_ll, c_double = C.c_void_p, C.c_int, C.c_longlong, C.c_double
 
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-class PagedDesc(C.Structure):
-    _fields_ = (
-        [("k_pages", c_void_p), ("v_pages", c_void_p)]
-        + [(f"{n}_stride_{a}", c_ll) for n in ("k", "v") for a in ("page", "head", "token")]
-        + [("table", c_void_p), ("table_stride", c_ll), ("lengths", c_void_p), ("offsets", c_void_p),
-           ("table_width", c_int), ("seqs", c_int), ("rows", c_int), ("pages", c_int), ("page_size", c_int),
-           ("Hq", c_int), ("Hkv", c_int), ("D", c_int), ("dtype", c_int), ("scale", c_float),
-           ("x", c_void_p), ("x_stride_row", c_ll), ("x_stride_head", c_ll),
-           ("out", c_void_p), ("workspace", c_void_p), ("status", c_void_p)]
-    )
-
+# incin_paged_desc of the C header, field by field in native alignment.  Packed as bytes: a ctypes structure of as many fields
+# takes three times as long to fill, which short calls notice.
+_pack_desc = struct.Struct("@PP6qPqPP9ifPqqPPP").pack
 
 nat.register_cuda_signatures({
-    "incin_kv_append": (c_int, [C.POINTER(PagedDesc), c_double, c_void_p]),
-    "incin_decode_attention_workspace": (c_ll, [C.POINTER(PagedDesc)]),
-    "incin_decode_attention": (c_int, [C.POINTER(PagedDesc), c_void_p]),
-    "incin_prompt_attention_workspace": (c_ll, [C.POINTER(PagedDesc)]),
-    "incin_prompt_attention": (c_int, [C.POINTER(PagedDesc), c_void_p]),
+    "incin_kv_append": (c_int, [c_void_p, c_double, c_void_p]),
+    "incin_decode_attention_workspace": (c_ll, [c_void_p]),
+    "incin_decode_attention": (c_int, [c_void_p, c_void_p]),
+    "incin_prompt_attention_workspace": (c_ll, [c_void_p]),
+    "incin_prompt_attention": (c_int, [c_void_p, c_void_p]),
     "incin_copy_pages": (c_int, [c_void_p] * 3 + [c_int, c_ll, c_int, c_ll, c_void_p, c_void_p]),
 })
 
@@ -55,10 +48,15 @@ _KIND = {torch.bfloat16: nat.GEMM_IN_BF16, torch.float16: nat.GEMM_IN_FP16}
 
 
 # ------------------------------------------------------------------------------------------------------------- checks
-def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int):
-    """The strides of the pages, once everything about the arguments is in order (these checks and the descriptor are most
-    of a short call's time: no attribute is asked for twice)."""
-    shape, dtype, device = k_pages.shape, x.dtype, x.device
+def _int_row(what: str, name: str, t, last: int) -> None:
+    if t.dtype is not torch.int32 or (last > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
+
+
+def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int) -> bool:
+    """Whether the kernels take the call (else the CPU does), once everything about the arguments is in order.  These checks
+    are a good part of a short call's time: no attribute is asked for twice."""
+    shape, dtype = k_pages.shape, x.dtype
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages must both be [pages, kv_heads, page_size, head_dim], got "
                          f"{tuple(shape)} and {tuple(v_pages.shape)}")
@@ -73,64 +71,55 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
     if len(t_shape) != 2 or len(l_shape) != 1 or t_shape[0] != l_shape[0] or t_shape[0] == 0 or t_shape[1] == 0:
         raise ValueError(f"{what}: table must be [sequences, entries] and lengths [sequences], got {tuple(t_shape)} and "
                          f"{tuple(l_shape)}")
-    seqs = t_shape[0]
+    seqs, width = t_shape
+    _int_row(what, "table", table, width)
+    _int_row(what, "lengths", lengths, seqs)
+    at = x.get_device()   # -1 on the CPU
+    if k_pages.get_device() != at or v_pages.get_device() != at or table.get_device() != at or lengths.get_device() != at:
+        raise ValueError(f"{what}: tensors on {[str(t.device) for t in (x, k_pages, v_pages, table, lengths)]}")
     if offsets is None:
         if rows != seqs:
             raise ValueError(f"{what}: {rows} rows for {seqs} sequences (one row each, or offsets)")
-    elif tuple(offsets.shape) != (seqs + 1,):
-        raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
-    for name, t in (("table", table), ("lengths", lengths), ("offsets", offsets)):
-        if t is not None and (t.dtype is not torch.int32 or (t.stride(-1) != 1 and t.shape[-1] > 1)):
-            raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
-    for t in (k_pages, v_pages, table, lengths, offsets):
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    else:
+        if offsets.dim() != 1 or offsets.shape[0] != seqs + 1:
+            raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
+        _int_row(what, "offsets", offsets, seqs + 1)
+        if offsets.get_device() != at:
+            raise ValueError(f"{what}: offsets on {offsets.device}, the others on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
-    if device.type != "cuda":
-        return None
+    if at < 0:
+        return False
     if dtype not in _KIND or D not in (64, 128):
         raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
     if n_heads // hkv > 128:
         raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
-    return _page_strides(what, "k_pages", k_pages) + _page_strides(what, "v_pages", v_pages)
+    return True
 
 
-def _page_strides(what: str, name: str, t) -> tuple[int, int, int]:
+def _page_strides(what: str, name: str, t, at: int) -> tuple[int, int, int]:
     a, b, c, d = t.stride()
-    if d != 1 or a % 8 or b % 8 or c % 8 or min(a, b, c) <= 0 or t.data_ptr() % 16:
+    if d != 1 or (a | b | c) % 8 or a <= 0 or b <= 0 or c <= 0 or at % 16:
         raise nat.NativeError(f"{what}: {name} needs contiguous rows that start on 16-byte boundaries, got strides {t.stride()}")
     return a, b, c
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """``x`` ``[rows, heads, head_dim]`` with contiguous heads that start on 16-byte boundaries, none of them shared."""
-    a, b, c = x.stride()
-    if c == 1 and a > 0 and b > 0 and not (a % 8 or b % 8 or x.data_ptr() % 16):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _launch(fn, what: str, x, k_pages, v_pages, table, lengths, offsets, strides, out, scale: float = 0.0, args=(), workspace=None):
+def _launch(fn, what: str, x, x_strides, k_pages, v_pages, table, lengths, offsets, n_heads: int, out, scale: float = 0.0, args=(), workspace=None):
     pages, hkv, size, D = k_pages.shape
     seqs, width = table.shape
-    x_row, x_head, _ = x.stride()
-    d = PagedDesc(k_pages.data_ptr(), v_pages.data_ptr(), *strides, table.data_ptr(), table.stride(0), lengths.data_ptr(),
-                  None if offsets is None else offsets.data_ptr(), width, seqs, x.shape[0], pages, size, out.shape[1], hkv, D,
-                  _KIND[x.dtype], scale, x.data_ptr(), x_row, x_head, out.data_ptr(), None, status_word(x.device).data_ptr())
-    at = C.byref(d)
-    room = None
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    fields = (k_at, v_at, *_page_strides(what, "k_pages", k_pages, k_at), *_page_strides(what, "v_pages", v_pages, v_at), table.data_ptr(),
+              table.stride(0), lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), width, seqs, x.shape[0], pages, size,
+              n_heads, hkv, D, _KIND[x.dtype], scale, x.data_ptr(), *x_strides, out.data_ptr())
+    status = status_word(x.device).data_ptr()
+    desc, room = _pack_desc(*fields, 0, status), None
     if workspace is not None:
-        n = workspace(at)
+        n = workspace(desc)
         if n:   # of this call alone: two captured graphs share none
-            room = torch.empty(n, dtype=torch.uint8, device=x.device)
-            d.workspace = room.data_ptr()
-    nat.check(fn(at, *args, nat.stream_ptr()), what)
+            room = x.new_empty(n, dtype=torch.uint8)
+            desc = _pack_desc(*fields, room.data_ptr(), status)
+    nat.check(fn(desc, *args, nat.stream_ptr()), what)
     return out
-
-
-def _is_current(t: torch.Tensor) -> bool:
-    return t.device.index == torch.cuda.current_device()
 
 
 # ------------------------------------------------------------------------------------------------------------- append
@@ -144,22 +133,23 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
     if k_pages.dim() != 4 or qkv.dim() != 2:
         raise ValueError(f"kv_append: qkv must be [rows, width] and k_pages [pages, kv_heads, page_size, head_dim], got "
                          f"{tuple(qkv.shape)} and {tuple(k_pages.shape)}")
-    rows, hkv, D = qkv.shape[0], k_pages.shape[1], k_pages.shape[3]
-    if qkv.shape[1] != (n_heads + 2 * hkv) * D or D % 2:
-        raise ValueError(f"kv_append: rows of {qkv.shape[1]} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
+    (rows, wide), (_, hkv, _, D) = qkv.shape, k_pages.shape
+    if wide != (n_heads + 2 * hkv) * D or D % 2:
+        raise ValueError(f"kv_append: rows of {wide} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
     if theta is not None and not 1.0 <= theta < 1e300:
         raise ValueError(f"kv_append: theta must be at least 1, got {theta}")
-    strides = _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
-    x = qkv.unflatten(1, (n_heads + 2 * hkv, D))
-    if not qkv.is_cuda:
-        return _append_cpu(x, k_pages, v_pages, table, lengths, offsets, n_heads, theta)
-    if not _is_current(qkv):
+    if not _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads):
+        return _append_cpu(qkv.unflatten(1, (n_heads + 2 * hkv, D)), k_pages, v_pages, table, lengths, offsets, n_heads, theta)
+    if qkv.get_device() != nat.device_index():
         with torch.cuda.device(qkv.device):
             return kv_append(qkv, k_pages, v_pages, table, lengths, offsets, n_heads=n_heads, theta=theta)
-    q = torch.empty(rows, n_heads, D, dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((rows, n_heads, D))
     if rows == 0:
         return q
-    return _launch(nat.cuda().incin_kv_append, "kv_append", _rows16(x), k_pages, v_pages, table, lengths, offsets, strides, q,
+    step, one = qkv.stride()
+    if one != 1 or step % 8 or step <= 0 or qkv.data_ptr() % 16:   # the kernel wants dense heads on 16-byte boundaries
+        qkv, step = qkv.clone(memory_format=torch.contiguous_format), wide
+    return _launch(nat.cuda().incin_kv_append, "kv_append", qkv, (step, D), k_pages, v_pages, table, lengths, offsets, n_heads, q,
                    args=(theta or 0.0,))
 
 
@@ -184,22 +174,25 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
         raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(q.shape)} and pages "
                          f"{tuple(k_pages.shape)}")
     rows, n_heads, D = q.shape
-    strides = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    native = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or scale < 0:
+    if not 0.0 <= scale < math.inf:
         raise ValueError(f"{what}: scale must be finite and not negative, got {scale}")
-    if not q.is_cuda:
+    if not native:
         return _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale)
-    if not _is_current(q):
+    if q.get_device() != nat.device_index():
         with torch.cuda.device(q.device):
             return _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale)
-    out = torch.empty(rows, n_heads, D, dtype=q.dtype, device=q.device)
+    out = q.new_empty((rows, n_heads, D))
     if rows == 0:
         return out
+    a, b, one = q.stride()
+    if one != 1 or (a | b) % 8 or a <= 0 or b <= 0 or q.data_ptr() % 16:   # the kernels want dense heads on 16-byte boundaries
+        q, a, b = q.clone(memory_format=torch.contiguous_format), n_heads * D, D
     lib = nat.cuda()
     fn, room = ((lib.incin_decode_attention, lib.incin_decode_attention_workspace) if offsets is None else
                 (lib.incin_prompt_attention, lib.incin_prompt_attention_workspace))
-    return _launch(fn, what, _rows16(q), k_pages, v_pages, table, lengths, offsets, strides, out, scale, workspace=room)
+    return _launch(fn, what, q, (a, b), k_pages, v_pages, table, lengths, offsets, n_heads, out, scale, workspace=room)
 
 
 # -------------------------------------------------------------------------------------------------------------- pages
@@ -239,7 +232,7 @@ def copy_pages(storage, src, dst):
         return storage
     if storage.data_ptr() % 16:
         raise nat.NativeError("copy_pages: storage must start on a 16-byte boundary")
-    if not _is_current(storage):
+    if storage.get_device() != nat.device_index():
         with torch.cuda.device(storage.device):
             return copy_pages(storage, src, dst)
     src, dst = src.contiguous(), dst.contiguous()

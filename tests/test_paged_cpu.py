@@ -232,3 +232,16 @@ def test_extending_equals_scoring_the_whole_text(kind):
         with pytest.raises(ValueError):
             model.extend(tokens, c, seqs, counts)
     assert c.length(b) == 50
+
+
+def test_descriptor_matches_the_header():
+    """The bytes that the front end packs are the C structure, field by field."""
+    import struct
+    from incin_b200.ffi import parse_headers
+    from incin_b200.ops import paged
+    fields = next(s.fields for s in parse_headers()[0] if s.name == "incin_paged_desc")
+    letter = lambda t: "P" if t.endswith("*") else {"long long": "q", "int": "i", "float": "f"}[t]
+    want = struct.Struct("@" + "".join(letter(t) for _, t, _ in fields))
+    packer = paged._pack_desc.__self__
+    values = list(range(1, len(fields) + 1))
+    assert packer.size == want.size and packer.pack(*values) == want.pack(*values)
