@@ -13,10 +13,16 @@
 // byte permutes.  P^T comes out of S^T by transposing 8 x 8 blocks between the lanes (movmatrix).  No shared memory, no
 // barrier in the loop: a warp asks for its next keys as soon as the present ones are used, and values likewise.
 //
-// Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal run of all
-// units, each warp 16 tokens of every one.  A pair of sequence and head that crosses CTAs leaves fp32 parts
-// (O, m, l), which a second kernel joins in a fixed order.  So the lengths are needed on the device only, one long
-// sequence uses all SMs, and a captured launch stays balanced whatever its lengths become.
+// Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal run
+// of all units, each warp 16 tokens of every one.  Where CTAs get several units, a pair of sequence and head has one more
+// than its tokens fill, since to begin and end one costs about as much (64 sequences of up to 4096, 32 / 4 heads of 64: CTAs
+// with short sequences took 27 us, the others 20; 31.2 -> 28.0 us in all).  A pair that crosses CTAs leaves fp32 parts (O, m, l),
+// which a second kernel joins in a fixed order.  So the lengths are needed on the device only, one long sequence uses all SMs,
+// and a captured launch stays balanced whatever its lengths become.
+//
+// Bytes of the cache a second, of a measured copy's 6.47 TB/s: 128 sequences of up to 8192 tokens, 24 / 8 heads of 128, 332 us,
+// 6.7 TB/s; one of 131071, 88.5 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 92 us, 5.8; 64 of them 28 us, 4.4.  What is left
+// is a chain at both ends: lengths, page numbers, first keys (4 us from the launch to the first product), and 3 us for the join.
 #include "paged.cuh"
 
 #include <math_constants.h>
@@ -96,10 +102,12 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   pdl_launch_dependents();
   pdl_wait();
 
-  {   // units in front of each sequence; one without tokens has a unit too, which writes its zeros
-    const int per = (c.seqs + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32), s0 = threadIdx.x * per;
+  const int head_blocks = c.Hkv * p.chunks;
+  int extra;   // units of a pair without tokens
+  {   // units in front of each sequence; one without tokens has one of them too, which writes its zeros
+    const int per = (c.seqs + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32), s0 = threadIdx.x * per, s1 = min(s0 + per, c.seqs);
     int sum = 0;
-    for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
+    for (int s = s0; s < s1; ++s) {
       length[s] = paged_length(c, s);
       sum += max(1, (length[s] + p.unit - 1) / p.unit);
     }
@@ -111,16 +119,20 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    int at = incl - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sum[w];
-    for (int s = s0; s < min(s0 + per, c.seqs); ++s) {
-      before[s] = at;
-      at += max(1, (length[s] + p.unit - 1) / p.unit);
-      if (s == c.seqs - 1) before[c.seqs] = at;
+    int at = incl - sum, all = 0;
+#pragma unroll
+    for (int w = 0; w < DEC_WARPS; ++w) {
+      if (w < warp) at += warp_sum[w];
+      all += warp_sum[w];
     }
+    extra = (long long)all * head_blocks > gridDim.x ? 1 : 0;   // where a CTA has a unit at most, all cost the same
+    for (int s = s0; s < s1; ++s) {
+      before[s] = at + s * extra;
+      at += max(1, (length[s] + p.unit - 1) / p.unit);
+    }
+    if (threadIdx.x == 0) before[c.seqs] = all + c.seqs * extra;
     __syncthreads();
   }
-  const int head_blocks = c.Hkv * p.chunks;
   const long long units = (long long)before[c.seqs] * head_blocks;
   const int ctas = (int)min((long long)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) {
@@ -140,16 +152,19 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     b = lo;
   }
 
-  // A run of units of one pair of sequence and key head.
-  int n_units, hb, t0, t1, key_end;
-  auto enter = [&](int& seq, long long unit) {
+  // A run of units of one pair of sequence and key head; the extra unit comes first.  Nothing is done for a run of that
+  // unit alone, the pair then begins in the next CTA (t0 is 1 there).
+  int n_units, hb, t0, t1, key_from, key_end;
+  auto enter = [&](int& seq, long long unit) -> bool {
     while ((long long)before[seq + 1] * head_blocks <= unit) ++seq;
     n_units = before[seq + 1] - before[seq];
     const long long rest = unit - (long long)before[seq] * head_blocks;
     hb = (rest >> 32) ? (int)(rest / n_units) : (int)((uint32_t)rest / (uint32_t)n_units);
     t0 = (int)(rest - (long long)hb * n_units);
     t1 = (int)min((long long)n_units, t0 + (u_end - unit));
-    key_end = (int)min((long long)length[seq], (long long)t1 * p.unit);
+    key_from = max(t0 - extra, 0) * p.unit;
+    key_end = (int)min((long long)length[seq], (long long)(t1 - extra) * p.unit);
+    return t1 > extra;
   };
   // 16 keys from a multiple of 16 on lie in one page.  A lane holds the page of one of the next 32 steps of its warp.
   auto pages_from = [&](int seq, int key) {
@@ -189,22 +204,25 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + row * c.v_token + j * 64 + r * 8, there);
     }
   };
-  enter(b, u);
-  pages = pages_from(b, t0 * p.unit + warp * 16);
+  if (!enter(b, u)) {
+    if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = opened;
+    return;
+  }
+  pages = pages_from(b, key_from + warp * 16);
   load_q();
-  load_k(t0 * p.unit + warp * 16, 0);
-  load_v(t0 * p.unit + warp * 16, 0);
+  load_k(key_from + warp * 16, 0);
+  load_v(key_from + warp * 16, 0);
 
   while (true) {
-    const int first = t0 * p.unit + warp * 16;
-    const long long next_u = u + (t1 - t0);
+    const int first = key_from + warp * 16;
+    long long next_u = u + (t1 - t0);
     int next_pages = -1;
     if (next_u < u_end) {   // asked for now, needed when this run ends
-      const int keep[5] = {n_units, hb, t0, t1, key_end};
+      const int keep[6] = {n_units, hb, t0, t1, key_from, key_end};
       int next_b = b;
-      enter(next_b, next_u);
-      next_pages = pages_from(next_b, t0 * p.unit + warp * 16);
-      n_units = keep[0], hb = keep[1], t0 = keep[2], t1 = keep[3], key_end = keep[4];
+      if (enter(next_b, next_u)) next_pages = pages_from(next_b, key_from + warp * 16);
+      else next_u = u_end;
+      n_units = keep[0], hb = keep[1], t0 = keep[2], t1 = keep[3], key_from = keep[4], key_end = keep[5];
     }
     float o[NT][VJ][4][4];
     float m[NT][2], l[NT][2];
@@ -299,8 +317,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       enter(b, u);
       pages = next_pages;
       load_q();
-      load_k(t0 * p.unit + warp * 16, 0);
-      load_v(t0 * p.unit + warp * 16, 0);
+      load_k(key_from + warp * 16, 0);
+      load_v(key_from + warp * 16, 0);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -321,8 +339,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       }
     __syncthreads();
     const int h0 = done_hb % p.chunks * Cfg::HEADS, first_head = done_hb / p.chunks * p.group + h0, heads = min(Cfg::HEADS, p.group - h0);
-    const bool whole = done_t0 == 0 && done_t1 == done_units;
-    float* slot = p.parts + (2ll * blockIdx.x + (done_t0 == 0)) * Cfg::SLOT;
+    const bool whole = done_t0 <= extra && done_t1 == done_units;
+    float* slot = p.parts + (2ll * blockIdx.x + (done_t0 <= extra)) * Cfg::SLOT;
     for (int i = threadIdx.x; i < Cfg::HEADS * (D / 8); i += DEC_WARPS * 32) {
       const int h = i / (D / 8), d = i % (D / 8) * 8;
       if (h >= heads) continue;
@@ -352,7 +370,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         }
       }
     }
-    if (done_t0 == 0 && !whole) {
+    if (done_t0 <= extra && !whole) {
       const long long last_unit = (long long)before[done_b] * head_blocks + (long long)(done_hb + 1) * done_units - 1;
       opened = make_int4(done_b, done_hb, (int)(((last_unit + 1) * ctas - 1) / units), 0);
     }
