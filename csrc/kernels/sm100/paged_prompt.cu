@@ -58,6 +58,7 @@ struct PrItem {
   int length;        // tokens of the sequence
   int lo, hi[2];     // K / V tiles [lo, hi[w]) for tile w
   int split;
+  int direct;        // the keys are not split after all: the first split writes the result itself
   int odd;           // set when a non-finite element of a late key was taken out of a V tile
 };
 
@@ -69,7 +70,7 @@ struct PrParams {
   int tiles;           // query tiles of an item: 2, or 1 where twice as many items are wanted
   int splits;
   float* part_o;       // [splits][rows][Hq][D]
-  float2* part_ml;     // [splits][rows][Hq]: m and l; l = -1 for a row without a position
+  float2* part_ml;     // [splits][rows][Hq]: m and l; l = -1 for a row without a position, -2 in the first split of one that is done
 };
 
 template <typename T>
@@ -247,9 +248,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             const int last = it.pos0 + min((w + 1) * p.tokens, it.tokens) - 1;
             n[w] = w < p.tiles && w * p.tokens < it.tokens && last >= 0 ? last / PR_BM + 1 : 0;
           }
-          const int most = max(n[0], n[1]);
-          it.lo = (int)((long long)most * it.split / p.splits);
-          const int hi = (int)((long long)most * (it.split + 1) / p.splits);
+          // the host splits by what the table holds; at least three tiles a split are worth it
+          const int most = max(n[0], n[1]), splits = min(p.splits, max(1, most / 3)), mine = min(it.split, splits);
+          it.direct = splits == 1;
+          it.lo = (int)((long long)most * mine / splits);
+          const int hi = (int)((long long)most * min(mine + 1, splits) / splits);
           it.hi[0] = min(hi, n[0]);
           it.hi[1] = min(hi, n[1]);
         }
@@ -577,10 +580,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const float l_sum = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
       const long long out_row = (long long)(it.row0 + mine) * c.Hq + it.head * p.group + g;
       const bool odd = ran && *reinterpret_cast<volatile int*>(&items[i % PR_ITEMS].odd);
-      const bool parts = p.splits > 1;
+      const bool parts = p.splits > 1 && !(it.direct && it.split == 0), empty_part = it.direct && it.split > 0;
       const float inv = limit < 0 ? 0.f : parts ? 1.f : 1.0f / l_sum;
 #pragma unroll 1
-      for (int ch = 0; ch < D / 32; ++ch) {
+      for (int ch = 0; ch < (empty_part ? 0 : D / 32); ++ch) {
         uint32_t o[32];
         if (ran) {
           tmem_ld_32x32(tmem_O + ch * 32, o);
@@ -627,7 +630,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         __syncwarp();
       }
-      if (live_row && parts) p.part_ml[(long long)it.split * c.rows * c.Hq + out_row] = make_float2(m_ref, limit < 0 ? -1.f : l_sum);
+      if (live_row && p.splits > 1)
+        p.part_ml[(long long)it.split * c.rows * c.Hq + out_row] = parts ? make_float2(m_ref, limit < 0 ? -1.f : l_sum) : make_float2(-CUDART_INF_F, -2.f);
       tc_fence_before();   // O_w has been read before the next item's first product, which follows this warp's p_part
       drop_item(i);
     }
@@ -660,6 +664,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
 #pragma unroll
   for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
   const float weight = ml.x == -CUDART_INF_F ? 0.f : ml.x == top ? 1.f : exp2f(ml.x - top);
+  if (__any_sync(0xffffffffu, ml.y == -2.f)) return;
   const bool nowhere = __any_sync(0xffffffffu, ml.y < 0.f);
   float sum = weight * ml.y, acc[PER] = {};
 #pragma unroll

@@ -296,6 +296,20 @@ def test_widest_groups(hq, hkv, D):
     _check_append(x, hq, k, v, table, lens, _i32(0, 3, 4, 144), 10000.0)
 
 
+@pytest.mark.parametrize("hq,hkv,D", [(24, 8, 128), (32, 4, 64)])
+@pytest.mark.parametrize("new,past", [([500], [0]), ([40, 3], [0, 900]), ([1, 0, 200], [0, 0, 5000])])
+def test_wide_tables(hq, hkv, D, new, past):
+    """Tables with room for far longer sequences, as a server keeps them for captured calls: entries behind the last token name
+    no page; how far the keys are split changes on the device."""
+    lengths = [a + b for a, b in zip(new, past)]
+    k, v, table, lens = make_cache(lengths, hkv, 16, D, torch.bfloat16, "cuda")
+    wide = torch.full((len(new), 8000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    offsets = _i32(0, *torch.tensor(new).cumsum(0).tolist())
+    _check_attention(_randn(sum(new) + 1, hq, D, dtype=torch.bfloat16, seed=15), k, v, wide, lens, offsets)
+    _check_attention(_randn(len(new), hq, D, dtype=torch.bfloat16, seed=16), k, v, wide, lens)
+
+
 def test_many_short_sequences():
     """More sequences than a warp, a launch or a table's rows hold at once; one table row for all of them."""
     hq, hkv, D = 8, 2, 64
