@@ -261,7 +261,7 @@ typedef struct incin_paged_desc {
   const void* x; /* attention: queries [rows, Hq, D]; append: projections [rows, Hq + 2 Hkv, D] */
   long long x_stride_row, x_stride_head;
   void* out; /* dense [rows, Hq, D] */
-  void* workspace; /* 16-byte aligned, as many bytes as the operation's _workspace function says; may be NULL for 0 */
+  void* workspace; /* 32-byte aligned, as many bytes as the operation's _workspace function says; may be NULL for 0 */
   void* status;
 } incin_paged_desc;
 /* Rotates queries and keys of the new rows to their positions (rotate-half pairs, theta > 0; 0 leaves them as they are),

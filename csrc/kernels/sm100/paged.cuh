@@ -36,7 +36,7 @@ inline int check_paged(const incin_paged_desc* d) {
   if (d->page_size != 16 && d->page_size != 32 && d->page_size != 64 && d->page_size != 128) return INCIN_ERR_UNSUPPORTED;
   if (d->D != 64 && d->D != 128) return INCIN_ERR_UNSUPPORTED;
   if (d->dtype != INCIN_GEMM_IN_BF16 && d->dtype != INCIN_GEMM_IN_FP16) return INCIN_ERR_UNSUPPORTED;
-  if (((uintptr_t)d->k_pages | (uintptr_t)d->v_pages | (uintptr_t)d->x | (uintptr_t)d->out | (uintptr_t)d->workspace) & 15)
+  if (((uintptr_t)d->k_pages | (uintptr_t)d->v_pages | (uintptr_t)d->x | (uintptr_t)d->out) & 15 || ((uintptr_t)d->workspace & 31))
     return INCIN_ERR_ALIGNMENT;
   const long long strides[] = {d->k_stride_page, d->k_stride_head, d->k_stride_token, d->v_stride_page, d->v_stride_head,
                                d->v_stride_token, d->x_stride_row, d->x_stride_head};

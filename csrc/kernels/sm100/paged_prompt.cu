@@ -610,10 +610,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
         }
         if (live_row && parts) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + ((long long)it.split * c.rows * c.Hq + out_row) * D + ch * 32);
+          float* dst = p.part_o + ((long long)it.split * c.rows * c.Hq + out_row) * D + ch * 32;   // whole sectors, as below
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            dst[u] = make_float4(__uint_as_float(o[u * 4]), __uint_as_float(o[u * 4 + 1]), __uint_as_float(o[u * 4 + 2]), __uint_as_float(o[u * 4 + 3]));
+          for (int u = 0; u < 4; ++u) st_global_b256(dst + u * 8, reinterpret_cast<uint32_t(&)[8]>(o[u * 8]));
         } else if (live_row) {
           uint32_t pk[16];
 #pragma unroll
@@ -699,7 +698,7 @@ struct PrPlan {
 // Query tiles of an item and CTAs that share its keys, by the time that the longest items take in all, in ns.  Measured at
 // head_dim 128 (24 / 8 heads) and 64 (32 / 4): a K / V tile takes a pair of query tiles 1580 and a single one 1460, an item's
 // beginning and end 1500, the joining kernel 3500 and its parts' bytes.  256 tokens behind 32768: single tiles and two splits
-// 214 us, pairs and four 130 us; 500 tokens alone: single tiles 14.1 us, pairs 15.0, two splits 25.8.
+// 214 us, pairs and four 126 us, nine 133; 500 tokens alone: single tiles 14.1 us, pairs 15.0, two splits 25.8.
 static PrPlan pr_plan(const incin_paged_desc* d) {
   PrPlan pl = {};
   const int sms = device_sm_count();
@@ -712,7 +711,7 @@ static PrPlan pr_plan(const incin_paged_desc* d) {
       if (splits > 1 && n > 2 * sms) break;
       const double rounds = n <= 3 * sms ? (double)((n + sms - 1) / sms) : (double)n / sms + 0.5;
       double time = rounds * ((double)((keys + splits - 1) / splits) * (tiles == 2 ? 1580 : 1460) + 1500);
-      if (splits > 1) time += 3500 + (double)splits * d->rows * d->Hq * d->D * 8 / 4000;
+      if (splits > 1) time += 3500 + (double)splits * d->rows * d->Hq * d->D * 8 / 2500;
       if (pl.tiles == 0 || time < best) best = time, pl.tiles = tiles, pl.splits = splits;
     }
   pl.items = ((long long)d->rows / (pl.tiles * pl.tokens) + d->seqs) * d->Hkv * pl.splits;   // at most
