@@ -18,6 +18,18 @@
 //   tiles that hold such keys before the product reads them: rows behind the sequence become zeros, and non-finite
 //   elements of keys that some row must not see become zeros and are added back, row by row, at the end (an item that had
 //   any reads them from the cache again; a weight is positive, so the element itself is what the sum takes from it).
+// - A CTA takes the next item when it has done its own (clusterlaunchcontrol: it takes over a CTA of the grid that has not
+//   started).  Dealt out in advance, 16 runs of 8000 tokens in all took 119 us in place of 102, 32 / 4 heads of 64.
+//
+// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 338 us, 1.22 PFLOP/s (the dense kernel 317-368 us by
+// the clock); 16 runs of 8000, 32 / 4 heads of 64, 103 us, 0.51; 256 tokens behind 32768, 125 us, 0.83; 37 tokens 7 us.
+// What bounds it: a K / V tile takes a pair of query tiles 1.5 to 1.6 us at either head_dim, of which the tensor pipe, the
+// special-function unit and tensor memory are each busy two thirds (ncu at head_dim 128: 63, 63 and 66 %); a warp's
+// row takes 1360-1480 clocks for its exponentials (1024 at the unit's rate), 500 for its maximum, and waits 620-930 for its scores.
+// Tried and slower, with that time in view: exponentials before the maximum is known (340 -> 355 us); the two warps of a
+// scheduler taking turns with theirs (331 -> 393 us at head_dim 64); P in columns of its own at head_dim 64 and the next scores
+// ahead of the product (331 -> 410); masked tiles without the products and exponentials of keys that no row sees (102 -> 118).
+// Without any maximum, as a limit, 1 % is gained.
 #include "paged.cuh"
 
 #include <math_constants.h>
