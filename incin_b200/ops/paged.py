@@ -5,7 +5,7 @@ with contiguous rows do).  Position ``j`` of sequence ``s`` lives in page ``tabl
 ``lengths[s]`` counts the tokens of the sequence with its new ones.  The new tokens of all sequences are packed rows: those of
 sequence ``s`` are rows ``offsets[s] .. offsets[s + 1]``, and they are its last tokens.  ``table``, ``lengths`` and ``offsets``
 are int32 tensors that are read on the device: no call synchronises, and a captured one follows their contents.  Entries of
-``table`` behind a sequence's last token and slots behind it are never read.  Rows outside every sequence, and sequences without
+``table`` behind a sequence's last token are not read, and what slots behind it hold has no effect.  Rows outside every sequence, and sequences without
 tokens, give zeros.
 
 On CUDA the tensors are bf16 or fp16 with head_dim 64 or 128, else the call is refused; the CPU takes any float type.  An
