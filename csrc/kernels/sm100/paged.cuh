@@ -65,17 +65,6 @@ __device__ __forceinline__ int paged_page(const PagedView& c, int s, int i) {
   flag_bad_index(c.status);
   return -1;
 }
-// First sequence whose rows end behind row t, or -1 when row t lies outside every sequence.
-__device__ __forceinline__ int paged_sequence(const PagedView& c, int t) {
-  if (!c.offsets) return t < c.seqs ? t : -1;
-  int lo = 0, hi = c.seqs;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (c.offsets[mid + 1] > t) hi = mid; else lo = mid + 1;
-  }
-  return lo < c.seqs && c.offsets[lo] <= t ? lo : -1;
-}
-
 struct Bf16 {
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return unpack_bf16x2(u); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }

@@ -483,14 +483,14 @@ static DecPlan dec_plan(const incin_paged_desc* d) {
   pl.chunks = (d->Hq / d->Hkv + Cfg::HEADS - 1) / Cfg::HEADS;
   const long long seqs = d->seqs < DEC_SEQS ? d->seqs : DEC_SEQS;
   const long long steps = ((long long)d->table_width * d->page_size + DEC_STEP - 1) / DEC_STEP;
-  // Where the table holds up to four steps, a pair stays with one CTA and the joining kernel is not needed: one sequence of 77
-  // tokens, 12 heads of 64, 6.0 -> 4.5 us.  (With eight steps the join is worth it: 8 sequences of up to 500, 32 / 4 heads of
-  // 64, 9.5 us a pair per CTA, 8.0 us split.)
-  const bool whole = steps <= 4;
+  const long long room = (long long)device_sm_count() * Cfg::CTAS_PER_SM, pairs = seqs * d->Hkv * pl.chunks;
+  // Where the table holds up to four steps and every pair has a CTA, it stays with it and the joining kernel is not needed: one
+  // sequence of 77 tokens, 12 heads of 64, 6.0 -> 4.5 us.  (With eight steps the join is worth it: 8 sequences of up to 500,
+  // 32 / 4 heads of 64, 9.5 us a pair per CTA, 8.0 us split.  With several pairs a CTA it is, too: 256 sequences of up to 250,
+  // 24 / 8 heads of 128, 42.7 us and 36.7.)
+  const bool whole = steps <= 4 && pairs <= room;
   pl.unit = DEC_STEP * (whole ? (int)steps : 1);
-  const long long per_pair = whole ? 1 : steps;
-  const long long most = seqs * d->Hkv * pl.chunks * per_pair;
-  const long long room = (long long)device_sm_count() * Cfg::CTAS_PER_SM;
+  const long long per_pair = whole ? 1 : steps, most = pairs * per_pair;
   pl.grid = (int)(most < room ? most : room);
   pl.splits = per_pair > 1;
   pl.bytes = pl.splits ? (long long)pl.grid * (16 + 2 * Cfg::SLOT * 4) : 0;
