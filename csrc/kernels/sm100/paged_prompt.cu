@@ -209,6 +209,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       // sequences [chunk, chunk + 32): a lane's items and those in front of them
       int chunk = -32, before = 0, total = 0, my_items = 0, my_upto = 0, my_row = 0, my_new = 0, my_len = 0;
       const int item_tokens = p.tiles * p.tokens;
+      // (offsets that overlap could name more items than fit; the grid has fewer indices)
+      auto most_items = [](int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); };
       // An item per CTA of the grid; CTAs that run take over those that have not started.
       int idx = (int)blockIdx.x;
       const int begin = min(max(c.offsets[0], 0), c.rows), end = min(max(c.offsets[c.seqs], begin), c.rows);
@@ -217,9 +219,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       int published = 0;
       while (ok) {
         if (idx >= 0 && idx < before) chunk = -32, before = total = 0;   // (indices come in rising order)
-        while (idx >= 0 && chunk < c.seqs && idx >= before + total) {
+        while (idx >= 0 && chunk < c.seqs && idx >= most_items(before, total)) {
           chunk += 32;
-          before += total;
+          before = most_items(before, total);
           const int s = chunk + lane;
           my_items = my_row = my_new = my_len = 0;
           if (s < c.seqs) {
@@ -233,7 +235,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
           for (int w = 1; w < 32; w <<= 1) {
             const int other = __shfl_up_sync(0xffffffffu, my_upto, w);
-            if (lane >= w) my_upto += other;
+            if (lane >= w) my_upto = most_items(my_upto, other);
           }
           total = __shfl_sync(0xffffffffu, my_upto, 31);
         }
