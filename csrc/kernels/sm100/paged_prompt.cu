@@ -29,7 +29,8 @@
 // row takes 1360-1480 clocks for its exponentials (1024 at the unit's rate), 500 for its maximum, and waits 620-930 for its scores.
 // Tried and slower, with that time in view: exponentials before the maximum is known (340 -> 355 us); the two warps of a
 // scheduler taking turns with theirs (331 -> 393 us at head_dim 64); P in columns of its own at head_dim 64 and the next scores
-// ahead of the product (331 -> 410); three regions for scores there, in turn, with the same aim (346 -> 361); masked tiles without the products and exponentials of keys that no row sees (102 -> 118).
+// ahead of the product (331 -> 410); three regions for scores there, in turn, with the same aim (346 -> 361); masked tiles
+// without the products and exponentials of keys that no row sees (102 -> 118).
 // Without any maximum, as a limit, 1 % is gained.
 #include "paged.cuh"
 
