@@ -248,7 +248,8 @@ int incin_flash_attn_bwd(const incin_attn_desc* desc, void* stream);
  * table, lengths and offsets are read on the device, so a captured launch follows their contents.  A length beyond the
  * table or an entry outside [0, pages) that is met writes KernelStatus 6 to *status; the entry reads as zeros and is not
  * written through.  Outputs of rows outside every sequence, and of sequences without tokens, are zeros.
- * Hq is a multiple of Hkv, Hq / Hkv at most 128. */
+ * Hq is a multiple of Hkv, Hq / Hkv at most 128.  A table holds up to 2^30 tokens a sequence; decode wants token strides
+ * below 2^23 elements. */
 typedef struct incin_paged_desc {
   void *k_pages, *v_pages;
   long long k_stride_page, k_stride_head, k_stride_token;

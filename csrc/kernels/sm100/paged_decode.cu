@@ -86,7 +86,7 @@ __device__ __forceinline__ void load16(uint32_t (&w)[4], const uint16_t* p, bool
 }
 
 // First unit of CTA i of n over `units` units
-__device__ __forceinline__ long long dec_start(long long units, int i, int n) { return units * i / n; }
+__device__ __forceinline__ int dec_start(int units, int i, int n) { return (int)((long long)units * i / n); }
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) decode_attention_kernel(const DecParams p) {
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       if (w < warp) at += warp_sum[w];
       all += warp_sum[w];
     }
-    extra = (long long)all * head_blocks > gridDim.x ? 1 : 0;   // where a CTA has a unit at most, all cost the same
+    extra = all * head_blocks > (int)gridDim.x ? 1 : 0;   // where a CTA has a unit at most, all cost the same
     for (int s = s0; s < s1; ++s) {
       before[s] = at + s * extra;
       at += max(1, (length[s] + p.unit - 1) / p.unit);
@@ -133,21 +133,21 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     if (threadIdx.x == 0) before[c.seqs] = all + c.seqs * extra;
     __syncthreads();
   }
-  const long long units = (long long)before[c.seqs] * head_blocks;
-  const int ctas = (int)min((long long)gridDim.x, units);
+  const int units = before[c.seqs] * head_blocks;   // (the host has seen to it that they fit)
+  const int ctas = min((int)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) {
     if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-  long long u = dec_start(units, blockIdx.x, ctas);
-  const long long u_end = dec_start(units, blockIdx.x + 1, ctas);
+  int u = dec_start(units, blockIdx.x, ctas);
+  const int u_end = dec_start(units, blockIdx.x + 1, ctas);
   int4 opened = make_int4(-1, 0, 0, 0);
   int b;   // the sequence of unit u
   {
     int lo = 0, hi = c.seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if ((long long)before[mid] * head_blocks <= u) lo = mid; else hi = mid - 1;
+      if (before[mid] * head_blocks <= u) lo = mid; else hi = mid - 1;
     }
     b = lo;
   }
@@ -155,53 +155,53 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   // A run of units of one pair of sequence and key head; the extra unit comes first.  Nothing is done for a run of that
   // unit alone, the pair then begins in the next CTA (t0 is 1 there).
   int n_units, hb, t0, t1, key_from, key_end;
-  auto enter = [&](int& seq, long long unit) -> bool {
-    while ((long long)before[seq + 1] * head_blocks <= unit) ++seq;
+  auto enter = [&](int& seq, int unit) -> bool {
+    while (before[seq + 1] * head_blocks <= unit) ++seq;
     n_units = before[seq + 1] - before[seq];
-    const long long rest = unit - (long long)before[seq] * head_blocks;
-    hb = (rest >> 32) ? (int)(rest / n_units) : (int)((uint32_t)rest / (uint32_t)n_units);
-    t0 = (int)(rest - (long long)hb * n_units);
-    t1 = (int)min((long long)n_units, t0 + (u_end - unit));
+    const unsigned rest = unit - before[seq] * head_blocks;
+    hb = rest / (unsigned)n_units;
+    t0 = rest - hb * n_units;
+    t1 = min(n_units, t0 + (u_end - unit));
     key_from = max(t0 - extra, 0) * p.unit;
-    key_end = (int)min((long long)length[seq], (long long)(t1 - extra) * p.unit);
+    key_end = min(length[seq], (t1 - extra) * p.unit);
     return t1 > extra;
   };
+  auto key_head = [&](int block) { return p.chunks == 1 ? block : block / p.chunks; };
+  auto first_of = [&](int block) { return p.chunks == 1 ? 0 : block % p.chunks * Cfg::HEADS; };   // query head of the group
   // 16 keys from a multiple of 16 on lie in one page.  A lane holds the page of one of the next 32 steps of its warp.
   auto pages_from = [&](int seq, int key) {
     const int mine = key + lane * DEC_STEP;
     return mine < key_end ? paged_page(c, seq, mine >> c.page_shift) : -1;
   };
+  // what a lane's rows and elements add to the first key's address; 16 rows of a page are less than 2^31 elements apart
+  const int k_token = (int)c.k_token, v_token = (int)c.v_token, k_lane = r * k_token + q4 * 8, v_lane = q4 * 2 * v_token + r * 8;
+  const int page_mask = (1 << c.page_shift) - 1;
   uint32_t q[NT][KJ][4], kr[2][KJ][4], vr[4][VJ][4];
   auto load_q = [&]() {
-    const int first_head = hb / p.chunks * p.group + hb % p.chunks * Cfg::HEADS, heads = p.group - hb % p.chunks * Cfg::HEADS;
+    const int h0 = first_of(hb), heads = p.group - h0;
+    const uint16_t* base = p.x + b * p.x_row + (key_head(hb) * p.group + h0 + r) * p.x_head + q4 * 8;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < KJ; ++j)
-        load16(q[t][j], p.x + b * p.x_row + (first_head + t * 8 + r) * p.x_head + j * 32 + q4 * 8, t * 8 + r < heads);
+      for (int j = 0; j < KJ; ++j) load16(q[t][j], base + t * 8 * p.x_head + j * 32, t * 8 + r < heads);
   };
   int pages;   // -1 where there is none
   auto load_k = [&](int key, int step) {
-    const uint16_t* kb = c.k + hb / p.chunks * c.k_head;
-    const int page = __shfl_sync(0xffffffffu, pages, step);
-    const uint16_t* base = kb + page * c.k_page + (key & ((1 << c.page_shift) - 1)) * c.k_token;
+    const int page = __shfl_sync(0xffffffffu, pages, step), left = page < 0 ? 0 : key_end - key;
+    const uint16_t* base = c.k + key_head(hb) * c.k_head + page * c.k_page + ((key & page_mask) * k_token + k_lane);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool there = page >= 0 && key + r + i * 8 < key_end;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) load16(kr[i][j], base + (r + i * 8) * c.k_token + j * 32 + q4 * 8, there);
-    }
+      for (int j = 0; j < KJ; ++j) load16(kr[i][j], base + (i * 8 * k_token + j * 32), r + i * 8 < left);
   };
   auto load_v = [&](int key, int step) {
-    const uint16_t* vb = c.v + hb / p.chunks * c.v_head;
-    const int page = __shfl_sync(0xffffffffu, pages, step);
-    const uint16_t* base = vb + page * c.v_page + (key & ((1 << c.page_shift) - 1)) * c.v_token;
+    const int page = __shfl_sync(0xffffffffu, pages, step), left = page < 0 ? 0 : key_end - key;
+    const uint16_t* base = c.v + key_head(hb) * c.v_head + page * c.v_page + ((key & page_mask) * v_token + v_lane);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = q4 * 2 + (i & 1) + (i >> 1) * 8;
-      const bool there = page >= 0 && key + row < key_end;
+      const int row = (i & 1) + (i >> 1) * 8;
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + row * c.v_token + j * 64 + r * 8, there);
+      for (int j = 0; j < VJ; ++j) load16(vr[i][j], base + (row * v_token + j * 64), q4 * 2 + row < left);
     }
   };
   if (!enter(b, u)) {
@@ -209,13 +209,79 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     return;
   }
   pages = pages_from(b, key_from + warp * 16);
-  load_q();
-  load_k(key_from + warp * 16, 0);
-  load_v(key_from + warp * 16, 0);
+  float o[NT][VJ][4][4], m[NT][2], l[NT][2];
+  int done_b = 0, done_hb = 0, done_t0 = 0, done_t1 = 0, done_units = 0, done_end = 0;
+  bool done = false;   // a run whose warps have to be joined
 
   while (true) {
+    // The queries and first keys and values of a run are on their way while the warps of the last one are joined.  (Asked for
+    // at one place in the code: with a second one in front of the loop the registers were copied, which waits for the data.)
+    const bool live = u < u_end;
+    if (live) {
+      load_q();
+      load_k(key_from + warp * 16, 0);
+      load_v(key_from + warp * 16, 0);
+    }
+    if (done) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], w);
+          if (r == 0) {
+            sm_m[warp][t * 8 + q4 * 2 + e] = m[t][e];
+            sm_l[warp][t * 8 + q4 * 2 + e] = l[t][e];
+          }
+#pragma unroll
+          for (int j = 0; j < VJ; ++j) {
+            float4* row = reinterpret_cast<float4*>(&sm_o[warp][t * 8 + q4 * 2 + e][j * 64 + r * 8]);
+            row[0] = make_float4(o[t][j][0][e], o[t][j][0][e + 2], o[t][j][1][e], o[t][j][1][e + 2]);
+            row[1] = make_float4(o[t][j][2][e], o[t][j][2][e + 2], o[t][j][3][e], o[t][j][3][e + 2]);
+          }
+        }
+      __syncthreads();
+      const int h0 = first_of(done_hb), first_head = key_head(done_hb) * p.group + h0, heads = min(Cfg::HEADS, p.group - h0);
+      const bool whole = done_t0 <= extra && done_t1 == done_units;
+      float* slot = p.parts + (2ll * blockIdx.x + (done_t0 <= extra)) * Cfg::SLOT;
+      for (int i = threadIdx.x; i < Cfg::HEADS * (D / 8); i += DEC_WARPS * 32) {
+        const int h = i / (D / 8), d = i % (D / 8) * 8;
+        if (h >= heads) continue;
+        float top = -CUDART_INF_F, sum = 0.f, acc[8] = {};
+#pragma unroll
+        for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, sm_m[w][h]);
+#pragma unroll
+        for (int w = 0; w < DEC_WARPS; ++w) {
+          // a warp without keys has m = -inf, l = 0 and O = 0
+          const float f = sm_m[w][h] == top ? 1.f : exp2f(sm_m[w][h] - top);
+          sum += f * sm_l[w][h];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += f * sm_o[w][h][d + e];
+        }
+        if (whole) {
+          const float inv = done_end > 0 ? 1.f / sum : 0.f;
+          *reinterpret_cast<uint4*>(p.out + ((long long)done_b * c.Hq + first_head + h) * D + d) =
+              make_uint4(T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv), T::pack(acc[4] * inv, acc[5] * inv),
+                         T::pack(acc[6] * inv, acc[7] * inv));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(slot + h * D + d);
+          dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          if (d == 0) {
+            slot[Cfg::HEADS * D + h] = top;
+            slot[Cfg::HEADS * (D + 1) + h] = sum;
+          }
+        }
+      }
+      if (done_t0 <= extra && !whole) {
+        const long long behind = (long long)before[done_b] * head_blocks + (done_hb + 1) * done_units;   // the pair's last unit + 1
+        opened = make_int4(done_b, done_hb, (int)((behind * ctas - 1) / units), 0);
+      }
+      if (!live) break;
+      __syncthreads();
+    }
     const int first = key_from + warp * 16;
-    long long next_u = u + (t1 - t0);
+    int next_u = u + (t1 - t0);
     int next_pages = -1;
     if (next_u < u_end) {   // asked for now, needed when this run ends
       const int keep[6] = {n_units, hb, t0, t1, key_from, key_end};
@@ -224,8 +290,6 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       else next_u = u_end;
       n_units = keep[0], hb = keep[1], t0 = keep[2], t1 = keep[3], key_from = keep[4], key_end = keep[5];
     }
-    float o[NT][VJ][4][4];
-    float m[NT][2], l[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t][0] = m[t][1] = -CUDART_INF_F;
@@ -310,72 +374,13 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
       if (next < key_end) load_v(next, step);
     }
 
-    // The keys, values and queries of the next run are on their way while the warps of this one are joined.
-    const int done_b = b, done_hb = hb, done_t0 = t0, done_t1 = t1, done_units = n_units, done_end = key_end;
+    done = true;
+    done_b = b, done_hb = hb, done_t0 = t0, done_t1 = t1, done_units = n_units, done_end = key_end;
     u = next_u;
     if (u < u_end) {
       enter(b, u);
       pages = next_pages;
-      load_q();
-      load_k(key_from + warp * 16, 0);
-      load_v(key_from + warp * 16, 0);
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], w);
-        if (r == 0) {
-          sm_m[warp][t * 8 + q4 * 2 + e] = m[t][e];
-          sm_l[warp][t * 8 + q4 * 2 + e] = l[t][e];
-        }
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) {
-          float4* row = reinterpret_cast<float4*>(&sm_o[warp][t * 8 + q4 * 2 + e][j * 64 + r * 8]);
-          row[0] = make_float4(o[t][j][0][e], o[t][j][0][e + 2], o[t][j][1][e], o[t][j][1][e + 2]);
-          row[1] = make_float4(o[t][j][2][e], o[t][j][2][e + 2], o[t][j][3][e], o[t][j][3][e + 2]);
-        }
-      }
-    __syncthreads();
-    const int h0 = done_hb % p.chunks * Cfg::HEADS, first_head = done_hb / p.chunks * p.group + h0, heads = min(Cfg::HEADS, p.group - h0);
-    const bool whole = done_t0 <= extra && done_t1 == done_units;
-    float* slot = p.parts + (2ll * blockIdx.x + (done_t0 <= extra)) * Cfg::SLOT;
-    for (int i = threadIdx.x; i < Cfg::HEADS * (D / 8); i += DEC_WARPS * 32) {
-      const int h = i / (D / 8), d = i % (D / 8) * 8;
-      if (h >= heads) continue;
-      float top = -CUDART_INF_F, sum = 0.f, acc[8] = {};
-#pragma unroll
-      for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, sm_m[w][h]);
-#pragma unroll
-      for (int w = 0; w < DEC_WARPS; ++w) {
-        // a warp without keys has m = -inf, l = 0 and O = 0
-        const float f = sm_m[w][h] == top ? 1.f : exp2f(sm_m[w][h] - top);
-        sum += f * sm_l[w][h];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += f * sm_o[w][h][d + e];
-      }
-      if (whole) {
-        const float inv = done_end > 0 ? 1.f / sum : 0.f;
-        *reinterpret_cast<uint4*>(p.out + ((long long)done_b * c.Hq + first_head + h) * D + d) =
-            make_uint4(T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv), T::pack(acc[4] * inv, acc[5] * inv),
-                       T::pack(acc[6] * inv, acc[7] * inv));
-      } else {
-        float4* dst = reinterpret_cast<float4*>(slot + h * D + d);
-        dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-        if (d == 0) {
-          slot[Cfg::HEADS * D + h] = top;
-          slot[Cfg::HEADS * (D + 1) + h] = sum;
-        }
-      }
-    }
-    if (done_t0 <= extra && !whole) {
-      const long long last_unit = (long long)before[done_b] * head_blocks + (long long)(done_hb + 1) * done_units - 1;
-      opened = make_int4(done_b, done_hb, (int)(((last_unit + 1) * ctas - 1) / units), 0);
-    }
-    if (u >= u_end) break;
-    __syncthreads();
   }
   if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = opened;
 }
@@ -502,7 +507,10 @@ static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
   using Cfg = DecCfg<D, NT>;
   const DecPlan pl = dec_plan<D, NT>(d);
   if (pl.splits && !d->workspace) return INCIN_ERR_ARGUMENT;
-  if ((long long)d->table_width * d->page_size > (1ll << 36) / DEC_SEQS) return INCIN_ERR_TOO_LARGE;   // units are counted in 32 bits
+  // units and the elements of 128 tokens are counted in 32 bits
+  const long long per_seq = ((long long)d->table_width * d->page_size / pl.unit + 2) * d->Hkv * pl.chunks;
+  if (per_seq >= (1ll << 30) || d->k_stride_token >= (1 << 23) || d->v_stride_token >= (1 << 23)) return INCIN_ERR_TOO_LARGE;
+  const int slice = (int)(per_seq * DEC_SEQS < (1ll << 31) ? DEC_SEQS : ((1ll << 31) - 1) / per_seq);
   DecParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
                  pl.unit, d->Hq / d->Hkv, pl.chunks, pl.splits ? (int4*)d->workspace : nullptr, (float*)((char*)d->workspace + 16ll * pl.grid)};
   p.c.offsets = nullptr;
@@ -510,9 +518,9 @@ static int launch_decode(const incin_paged_desc* d, cudaStream_t stream) {
   if (!shared_split(decode_attention_kernel<T, D, NT>, Cfg::SHARED, main_set) || !shared_split(decode_join_kernel<T, D, NT, 1>, Cfg::SHARED, join_set) ||
       !shared_split(decode_join_kernel<T, D, NT, 8>, Cfg::SHARED, wide_join_set))
     return INCIN_ERR_LAUNCH;
-  for (int s0 = 0; s0 < d->seqs; s0 += DEC_SEQS) {
+  for (int s0 = 0; s0 < d->seqs; s0 += slice) {
     DecParams q = p;
-    q.c.seqs = q.c.rows = d->seqs - s0 < DEC_SEQS ? d->seqs - s0 : DEC_SEQS;
+    q.c.seqs = q.c.rows = d->seqs - s0 < slice ? d->seqs - s0 : slice;
     q.c.table += s0 * d->table_stride;
     q.c.lengths += s0;
     q.x += s0 * d->x_stride_row;
