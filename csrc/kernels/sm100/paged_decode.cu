@@ -16,12 +16,12 @@
 // Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal run
 // of all units, each warp 16 tokens of every one.  Where CTAs get several units, a pair of sequence and head has one more
 // than its tokens fill, since to begin and end one costs about as much (64 sequences of up to 4096, 32 / 4 heads of 64: CTAs
-// with short sequences took 27 us, the others 20; 31.2 -> 28.0 us in all).  A pair that crosses CTAs leaves fp32 parts (O, m, l),
+// with short sequences took 27 us, the others 20; 31.2 -> 28.0 us in all when it was added).  A pair that crosses CTAs leaves fp32 parts (O, m, l),
 // which a second kernel joins in a fixed order.  So the lengths are needed on the device only, one long sequence uses all SMs,
 // and a captured launch stays balanced whatever its lengths become.
 //
-// Bytes of the cache a second, of a measured copy's 6.47 TB/s: 128 sequences of up to 8192 tokens, 24 / 8 heads of 128, 332 us,
-// 6.7 TB/s; one of 131071, 88.5 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 92 us, 5.8; 64 of them 28 us, 4.4.  What is left
+// Bytes of the cache a second, of a measured copy's 6.47 TB/s: 128 sequences of up to 8192 tokens, 24 / 8 heads of 128, 334 us,
+// 6.7 TB/s; one of 131071, 88.7 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 87.6 us, 6.1; 64 of them 26.4 us, 4.6.  What is left
 // is a chain at both ends: lengths, page numbers, first keys (4 us from the launch to the first product), and 3 us for the join.
 #include "paged.cuh"
 
@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   __shared__ int before[DEC_SEQS + 1];   // units of one head in front of each sequence
   __shared__ int length[DEC_SEQS];
   __shared__ int warp_sum[DEC_WARPS];
+  __shared__ __align__(16) int next_run[DEC_WARPS][8];
   __shared__ float sm_m[DEC_WARPS][Cfg::HEADS], sm_l[DEC_WARPS][Cfg::HEADS];
   __shared__ __align__(16) float sm_o[DEC_WARPS][Cfg::HEADS][Cfg::ROW];
   const PagedView& c = p.c;
@@ -214,8 +215,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
   bool done = false;   // a run whose warps have to be joined
 
   while (true) {
-    // The queries and first keys and values of a run are on their way while the warps of the last one are joined.  (Asked for
-    // at one place in the code: with a second one in front of the loop the registers were copied, which waits for the data.)
+    // The queries and first keys and values of a run are on their way while the warps of the last one are joined.
     const bool live = u < u_end;
     if (live) {
       load_q();
@@ -283,11 +283,15 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     const int first = key_from + warp * 16;
     int next_u = u + (t1 - t0);
     int next_pages = -1;
-    if (next_u < u_end) {   // asked for now, needed when this run ends
+    if (next_u < u_end) {   // asked for now, needed when this run ends; kept in shared memory: working it out again cost 3 % of 256 short pairs
       const int keep[6] = {n_units, hb, t0, t1, key_from, key_end};
       int next_b = b;
       if (enter(next_b, next_u)) next_pages = pages_from(next_b, key_from + warp * 16);
       else next_u = u_end;
+      if (lane == 0) {   // worked out once
+        *reinterpret_cast<int4*>(next_run[warp]) = make_int4(n_units, hb, t0, t1);
+        *reinterpret_cast<int4*>(next_run[warp] + 4) = make_int4(key_from, key_end, next_b, 0);
+      }
       n_units = keep[0], hb = keep[1], t0 = keep[2], t1 = keep[3], key_from = keep[4], key_end = keep[5];
     }
 #pragma unroll
@@ -378,7 +382,9 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     done_b = b, done_hb = hb, done_t0 = t0, done_t1 = t1, done_units = n_units, done_end = key_end;
     u = next_u;
     if (u < u_end) {
-      enter(b, u);
+      __syncwarp();
+      const int4 run = *reinterpret_cast<const int4*>(next_run[warp]), more = *reinterpret_cast<const int4*>(next_run[warp] + 4);
+      n_units = run.x, hb = run.y, t0 = run.z, t1 = run.w, key_from = more.x, key_end = more.y, b = more.z;
       pages = next_pages;
     }
   }
