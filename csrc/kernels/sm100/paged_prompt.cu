@@ -2,8 +2,11 @@
 //
 // One persistent CTA per SM works on items: up to two 128-row query tiles of one sequence and key head, over a range of its
 // keys.  The rows of a tile are (new token, query head of the key head), so that grouped heads share every key that is
-// loaded and a run of a few tokens still fills a tile: with G query heads a key head a tile holds 128 / G tokens.  A box of
-// the query map is {64 elements, G heads, 128 / G tokens}, one copy a half.  K and V tiles are 128 keys, fetched page
+// loaded and a run of a few tokens still fills a tile: with G query heads a key head a tile holds 128 / G tokens.  Where that is
+// not a whole number two tiles share the heads of a token (256 tokens of 24 / 8 heads fill 6 tiles in place of 7: 126 -> 99 us
+// behind 32768; 8191 alone 335 -> 325).  A box of the query map is {64 elements, G heads, the tokens that lie whole in a tile},
+// one copy a half; the shared tokens' rows are fetched by the two warps that otherwise look over V tiles (by one-row copies they
+// cost 2 us a tile at G = 12).  K and V tiles are 128 keys, fetched page
 // by page (a box is one page of one head); the lanes of the producer warp hold the page numbers.
 //
 // The arithmetic and its schedule are those of the dense causal kernel (attention_fwd.cu): S_w = Q_w K^T into tensor memory, a
@@ -67,7 +70,8 @@ struct PrCfg {
 
 struct PrItem {
   int seq, head;     // key head; -1 ends the list
-  int row0, tokens;  // first packed row of tile 0, new tokens from there to the end of the sequence's run
+  int row0, tokens;  // packed row of tile 0's first token, new tokens from there to the end of the sequence's run
+  int head0;         // query head of the key head in tile 0's first row
   int pos0;          // position of that token (negative: more new tokens than the sequence has)
   int length;        // tokens of the sequence
   int lo, hi[2];     // K / V tiles [lo, hi[w]) for tile w
@@ -78,9 +82,15 @@ struct PrItem {
 
 struct PrParams {
   PagedView c;
+  const uint16_t* x;
+  long long x_row, x_head;
   uint16_t* out;
   float scale_log2;
-  int group, tokens;   // query heads of a key head, tokens of a tile
+  int group;           // query heads of a key head
+  uint32_t by_group;   // n / group = n by_group >> (31 + by_shift) for 0 <= n < 2^31: 2^by_shift is the next power of two from
+  int by_shift;        // group on, by_group = 2^(31 + by_shift) / group, rounded up, so that the excess stays below 1 / group
+  int tile_rows;       // rows of a tile that are used
+  int box_tokens;      // tokens of tmQ's box
   int tiles;           // query tiles of an item: 2, or 1 where twice as many items are wanted
   int splits;
   float* part_o;       // [splits][rows][Hq][D]
@@ -144,6 +154,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 
   const PagedView& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto by_group = [&](int n) { return (int)(__umulhi(2u * (uint32_t)n, p.by_group) >> p.by_shift); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 4; ++s) {
@@ -154,7 +165,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(&clean[s], 2);
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&q_full[w], 1);
+      mbar_init(&q_full[w], 3);   // the box, single rows by two warps
       mbar_init(&q_empty[w], 1);
       mbar_init(&s_full[w], 1);
       mbar_init(&p_full[w], 4);
@@ -208,8 +219,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       bool ok = true;
       const int per_tile = PR_BM >> c.page_shift;   // pages of a K / V tile
       // sequences [chunk, chunk + 32): a lane's items and those in front of them
-      int chunk = -32, before = 0, total = 0, my_items = 0, my_upto = 0, my_row = 0, my_new = 0, my_len = 0;
-      const int item_tokens = p.tiles * p.tokens;
+      int chunk = -32, before = 0, total = 0, my_items = 0, my_pairs = 0, my_upto = 0, my_row = 0, my_new = 0, my_len = 0;
+      const int item_rows = p.tiles * p.tile_rows, group = p.group, per = c.Hkv * p.splits;
       // (offsets that overlap could name more items than fit; the grid has fewer indices)
       auto most_items = [](int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); };
       // An item per CTA of the grid; CTAs that run take over those that have not started.
@@ -224,13 +235,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           chunk += 32;
           before = most_items(before, total);
           const int s = chunk + lane;
-          my_items = my_row = my_new = my_len = 0;
+          my_items = my_pairs = my_row = my_new = my_len = 0;
           if (s < c.seqs) {
             my_row = min(max(c.offsets[s], 0), c.rows);
             my_new = min(max(c.offsets[s + 1], my_row), c.rows) - my_row;
             my_len = paged_length(c, s);
             if (my_new > my_len) flag_bad_index(c.status);
-            my_items = (my_new + item_tokens - 1) / item_tokens * c.Hkv * p.splits;
+            my_pairs = (my_new * group + item_rows - 1) / item_rows;
+            my_items = my_pairs * per;
           }
           my_upto = my_items;
 #pragma unroll
@@ -246,23 +258,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         if (there) {
           const int at = idx - before;
           const int owner = __ffs(__ballot_sync(0xffffffffu, at < my_upto)) - 1;
-          const int first = __shfl_sync(0xffffffffu, my_upto - my_items, owner), runs = __shfl_sync(0xffffffffu, my_items, owner);
+          const int first = __shfl_sync(0xffffffffu, my_upto - my_items, owner), pairs = __shfl_sync(0xffffffffu, my_pairs, owner);
           const int row = __shfl_sync(0xffffffffu, my_row, owner), fresh = __shfl_sync(0xffffffffu, my_new, owner);
           it.length = __shfl_sync(0xffffffffu, my_len, owner);
           it.seq = chunk + owner;
-          const int per = c.Hkv * p.splits, rest = at - first;
-          const int pair = runs / per - 1 - rest / per, k = rest % per;   // the longest first
-          it.head = k / p.splits;
-          it.split = k % p.splits;
-          const int t0 = pair * item_tokens;
+          const int rest = at - first, behind = rest / per, k = rest - behind * per;
+          const int pair = pairs - 1 - behind;   // the longest first
+          it.head = p.splits == 1 ? k : k / p.splits;
+          it.split = k - it.head * p.splits;
+          const int t0 = by_group(pair * item_rows);
+          it.head0 = pair * item_rows - t0 * group;
           it.row0 = row + t0;
           it.tokens = fresh - t0;
           it.pos0 = it.length - fresh + t0;
           int n[2];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {   // tiles up to the last row's own position
-            const int last = it.pos0 + min((w + 1) * p.tokens, it.tokens) - 1;
-            n[w] = w < p.tiles && w * p.tokens < it.tokens && last >= 0 ? last / PR_BM + 1 : 0;
+            const int at0 = it.head0 + w * p.tile_rows, last = it.pos0 + min(by_group(at0 + p.tile_rows - 1), it.tokens - 1);
+            n[w] = w < p.tiles && by_group(at0) < it.tokens && last >= 0 ? last / PR_BM + 1 : 0;
           }
           // the host splits by what the table holds; at least three tiles a split are worth it
           const int most = max(n[0], n[1]), splits = min(p.splits, max(1, most / 3)), mine = min(it.split, splits);
@@ -295,11 +308,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         auto load_q = [&](int w) -> bool {
           if (!mbar_wait(&q_empty[w], q_phase[w] ^ 1, abort_flag, c.status, kStatusTimeoutEmpty)) return false;
           q_phase[w] ^= 1;
+          const int at0 = it.head0 + w * p.tile_rows, first_token = by_group(at0), first_head = at0 - first_token * group;
+          const int front = first_head ? group - first_head : 0;
           if (leader) {
-            mbar_expect_tx(&q_full[w], p.group * p.tokens * D * 2);
+            mbar_expect_tx(&q_full[w], p.box_tokens * group * D * 2);
 #pragma unroll
             for (int ch = 0; ch < D / 64; ++ch)
-              tma_load_4d(smem + w * Cfg::TILE_BYTES + ch * (PR_BM * 128), &tmQ, &q_full[w], ch * 64, it.head * p.group, it.row0 + w * p.tokens, 0);
+              tma_load_4d(smem + w * Cfg::TILE_BYTES + ch * (PR_BM * 128) + front * 128, &tmQ, &q_full[w], ch * 64, it.head * group,
+                          it.row0 + first_token + (front > 0), 0);
           }
           __syncwarp();
           return true;
@@ -447,12 +463,34 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         drop_item(i);
       }
     } else {
-      // ---------------------------------------------------------------- V tiles with late keys: 64 threads, two rows each
+      // ---------------------------------------------------------------- V tiles with late keys, and single query rows: 64 threads
       const int tid = (warp - 2) * 32 + lane;
+      uint32_t q_phase = 0;   // a bit a tile
       PrRing<Cfg::V_STAGES> v_at;
       bool ok = true;
       PrItem it;
       for (int i = 0; ok && take_item(i, it); ++i) {
+        // query rows in front of the box and behind it: heads of tokens that two tiles share
+#pragma unroll 1
+        for (int w = 0; w < 2 && ok; ++w) {
+          if ((w ? it.hi[1] : it.hi[0]) <= it.lo) continue;
+          ok = mbar_wait(&q_empty[w], (q_phase >> w & 1) ^ 1, abort_flag, c.status, kStatusTimeoutEmpty);
+          if (!ok) break;
+          q_phase ^= 1 << w;
+          const int at0 = it.head0 + w * p.tile_rows, first_head = at0 - by_group(at0) * p.group;
+          const int front = first_head ? p.group - first_head : 0, boxed = p.box_tokens * p.group;
+          const int rows = front + min(max(it.tokens * p.group - at0 - front - boxed, 0), p.tile_rows - front - boxed);
+#pragma unroll 4
+          for (int i = tid; i < rows * (D / 8); i += 64) {
+            const int u = i % (D / 8), r = i / (D / 8) < front ? i / (D / 8) : i / (D / 8) + boxed, token = by_group(at0 + r);
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.x + (it.row0 + token) * p.x_row +
+                                                                 (it.head * p.group + at0 + r - token * p.group) * p.x_head + u * 8));
+            *reinterpret_cast<uint4*>(smem + w * Cfg::TILE_BYTES + (u >> 3) * (PR_BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = x;
+          }
+          if (rows) fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[w]);
+        }
         const int hi = max(it.hi[0], it.hi[1]), late = late_from(it);
         for (int j = it.lo; j < hi && ok; ++j) {
           const int v_stage = v_at.stage;
@@ -503,7 +541,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const int w = (warp >> 2) - 1;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // row inside the tile == TMEM lane
-    const int token = row / p.group, g = row - token * p.group;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tmem_S = tmem_base + w * PR_BM + lane_addr, tmem_O = tmem_base + Cfg::COL_O + w * D + lane_addr;
     uint32_t s_phase = 0, o_phase = 0;
@@ -511,10 +548,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     PrItem it;
     for (int i = 0; ok && take_item(i, it); ++i) {
       const int lo = it.lo, hi = it.hi[w];
-      const int mine = w * p.tokens + token;                     // token of the item
-      const bool live_row = w < p.tiles && token < p.tokens && mine < it.tokens;
-      const int limit = it.pos0 + (live_row ? mine : min(w * p.tokens, it.tokens - 1));   // the last key that the row sees
-      const int all_see = it.pos0 + w * p.tokens;                // ... and the last one that every row of the tile sees
+      const int at0 = it.head0 + w * p.tile_rows, first_token = by_group(at0);
+      const int mine = by_group(at0 + row), g = at0 + row - mine * p.group;   // token of the item and its query head
+      const bool live_row = w < p.tiles && row < p.tile_rows && mine < it.tokens;
+      const int limit = it.pos0 + (live_row ? mine : min(first_token, it.tokens - 1));   // the last key that the row sees
+      const int all_see = it.pos0 + first_token;                 // ... and the last one that every row of the tile sees
       float m_ref = -CUDART_INF_F;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = lo; j < hi; ++j) {
@@ -707,7 +745,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
 }
 
 struct PrPlan {
-  int tokens, tiles, splits;
+  int tile_rows, box_tokens, tiles, splits;
   long long items, bytes;
 };
 
@@ -718,19 +756,26 @@ struct PrPlan {
 static PrPlan pr_plan(const incin_paged_desc* d) {
   PrPlan pl = {};
   const int sms = device_sm_count();
-  pl.tokens = PR_BM / (d->Hq / d->Hkv);
+  const int group = d->Hq / d->Hkv;
+  // Groups that do not divide 128 fill all rows of a tile, too, up to 2 group - 2 of them one by one.  Large groups keep to whole
+  // tokens.  Whole and shared, one run of 6000, two key heads of 128: 3 heads each 86.3 and 85.8 us, 12: 194 and 184, 24: 380 and
+  // 363, 40: 640 and 608; one of 1000: 18.8 and 18.2, 22.7 and 22.6, 25.3 and 25.5, 39.7 and 44.8.
+  const bool dense = PR_BM % group != 0 && group <= 24;
+  pl.box_tokens = dense ? (PR_BM - group + 1) / group : PR_BM / group;
+  pl.tile_rows = dense ? PR_BM : pl.box_tokens * group;
+  const long long rows = (long long)d->rows * group;
   const long long keys = ((long long)d->table_width * d->page_size + PR_BM - 1) / PR_BM;   // K / V tiles of a sequence at most
   double best = 0;
   for (int tiles = 1; tiles <= 2; ++tiles)
     for (int splits = 1; splits <= 32 && (splits == 1 || splits * 2 <= keys); ++splits) {
-      const long long n = (((long long)d->rows + tiles * pl.tokens - 1) / (tiles * pl.tokens) + (d->seqs - 1) / 2) * d->Hkv * splits;
+      const long long n = ((rows + tiles * pl.tile_rows - 1) / (tiles * pl.tile_rows) + (d->seqs - 1) / 2) * d->Hkv * splits;
       if (splits > 1 && n > 2 * sms) break;
       const double rounds = n <= 3 * sms ? (double)((n + sms - 1) / sms) : (double)n / sms + 0.5;
       double time = rounds * ((double)((keys + splits - 1) / splits) * (tiles == 2 ? 1580 : 1460) + 1500);
       if (splits > 1) time += 3500 + (double)splits * d->rows * d->Hq * d->D * 8 / 2500;
       if (pl.tiles == 0 || time < best) best = time, pl.tiles = tiles, pl.splits = splits;
     }
-  pl.items = ((long long)d->rows / (pl.tiles * pl.tokens) + d->seqs) * d->Hkv * pl.splits;   // at most
+  pl.items = (rows / (pl.tiles * pl.tile_rows) + d->seqs) * d->Hkv * pl.splits;   // at most
   pl.bytes = pl.splits > 1 ? (long long)pl.splits * d->rows * d->Hq * (d->D * 4 + 8) : 0;
   return pl;
 }
@@ -739,11 +784,11 @@ template <typename T, int D>
 static int launch_prompt(const incin_paged_desc* d, cudaStream_t stream) {
   using Cfg = PrCfg<D>;
   const PrPlan pl = pr_plan(d);
-  if (pl.items > (1ll << 30)) return INCIN_ERR_TOO_LARGE;   // the kernel counts items in 32 bits
+  if (pl.items > (1ll << 30) || (long long)d->rows * (d->Hq / d->Hkv) > 0x7fffff00) return INCIN_ERR_TOO_LARGE;   // counted in 32 bits
   if (pl.bytes && !d->workspace) return INCIN_ERR_ARGUMENT;
   const int group = d->Hq / d->Hkv;
   CUtensorMap tq, tk, tv;
-  int rc = make_operand_map_box(&tq, d->x, D, d->Hq, d->Hq > 1 ? d->x_stride_head : D, d->rows, d->x_stride_row, 1, 0, 64, group, pl.tokens);
+  int rc = make_operand_map_box(&tq, d->x, D, d->Hq, d->Hq > 1 ? d->x_stride_head : D, d->rows, d->x_stride_row, 1, 0, 64, group, pl.box_tokens);
   if (rc) return rc;
   rc = make_operand_map(&tk, d->k_pages, D, d->page_size, d->k_stride_token, d->Hkv, d->k_stride_head, d->pages, d->k_stride_page, 64, d->page_size);
   if (rc) return rc;
@@ -753,7 +798,10 @@ static int launch_prompt(const incin_paged_desc* d, cudaStream_t stream) {
   static PerDeviceFlags attr;
   if (!ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr)) return INCIN_ERR_LAUNCH;
   const long long n = (long long)d->rows * d->Hq;
-  const PrParams p = {paged_view(d), (uint16_t*)d->out, d->scale * 1.4426950408889634f, group, pl.tokens, pl.tiles, pl.splits,
+  int by_shift = 0;
+  while (1 << by_shift < group) ++by_shift;
+  const PrParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
+                      group, (uint32_t)(((1ull << (31 + by_shift)) + group - 1) / group), by_shift, pl.tile_rows, pl.box_tokens, pl.tiles, pl.splits,
                       (float*)d->workspace, (float2*)((float*)d->workspace + pl.splits * n * D)};
   if (launch_pdl<true>(kern, dim3((unsigned)pl.items), dim3(PR_THREADS), Cfg::SMEM_BYTES, stream, tq, tk, tv, p) != cudaSuccess)
     return INCIN_ERR_LAUNCH;

@@ -215,6 +215,17 @@ def test_prompt_shapes(new, past, hq, hkv, D):
     _check_attention(q, k, v, table, lens, offsets)
 
 
+@pytest.mark.parametrize("group", [3, 5, 7, 11, 12, 13, 15, 17, 24, 40])
+@pytest.mark.parametrize("new,past", [([1, 9, 60], [0, 300, 0]), ([256], [5000]), ([333, 0, 1024], [0, 70, 129])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_groups_across_tiles(group, new, past, D):
+    """Groups that do not divide the rows of a query tile: tokens whose heads lie in two tiles, first and last rows of a run."""
+    lengths = [a + b for a, b in zip(new, past)]
+    k, v, table, lens = make_cache(lengths, 2, 16, D, torch.bfloat16, "cuda")
+    q = _randn(sum(new), 2 * group, D, dtype=torch.bfloat16, seed=24)
+    _check_attention(q, k, v, table, lens, _i32(0, *torch.tensor(new).cumsum(0).tolist()))
+
+
 @pytest.mark.parametrize("hq,hkv,D", [(12, 12, 64), (32, 4, 64), (24, 8, 128)])
 @pytest.mark.parametrize("at", [0, 5, 127, 128, 200, 299])
 def test_prompt_later_tokens_stay_out(hq, hkv, D, at):
