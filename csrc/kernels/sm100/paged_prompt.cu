@@ -24,16 +24,17 @@
 // - A CTA takes the next item when it has done its own (clusterlaunchcontrol: it takes over a CTA of the grid that has not
 //   started).  Dealt out in advance, 16 runs of 8000 tokens in all took 119 us in place of 102, 32 / 4 heads of 64.
 //
-// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 335 us, 1.23 PFLOP/s, in short bursts, 384 us for seconds
-// under the power cap (1642 MHz, 990 W; the dense kernel 317 and 368); 16 runs of 8000, 32 / 4 heads of 64, 103 us, 0.51 (1965 MHz,
-// 840 W); 256 tokens behind 32768, 125 us, 0.83 (142 under the cap, 1762 MHz); 37 tokens 7 us.
+// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 326 us, 1.26 PFLOP/s, in short bursts, more for seconds
+// under the power cap (990 W; the dense kernel 317 and 368); 16 runs of 8000 in all, 32 / 4 heads of 64, 105 us, 0.50 (1965 MHz,
+// 840 W); 256 tokens behind 32768, 24 / 8 heads of 128, 99 us, 1.04; 37 tokens 7 us.
 // What bounds it: a K / V tile takes a pair of query tiles 1.5 to 1.6 us at either head_dim, of which the tensor pipe, the
 // special-function unit and tensor memory are each busy two thirds (ncu at head_dim 128: 63, 63 and 66 %); a warp's
 // row takes 1360-1480 clocks for its exponentials (1024 at the unit's rate), 500 for its maximum, and waits 620-930 for its scores.
 // Tried and slower, with that time in view: exponentials before the maximum is known (340 -> 355 us); the two warps of a
 // scheduler taking turns with theirs (331 -> 393 us at head_dim 64); P in columns of its own at head_dim 64 and the next scores
 // ahead of the product (331 -> 410); three regions for scores there, in turn, with the same aim (346 -> 361); masked tiles
-// without the products and exponentials of keys that no row sees (102 -> 118).
+// without the products and exponentials of keys that no row sees (102 -> 118); an eighth of the exponentials by a polynomial on the
+// multiply-add units (326 -> 337, a quarter 342).
 // Without any maximum, as a limit, 1 % is gained.
 #include "paged.cuh"
 
