@@ -799,9 +799,11 @@ static int launch_prompt(const incin_paged_desc* d, cudaStream_t stream) {
   static PerDeviceFlags attr;
   if (!ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr)) return INCIN_ERR_LAUNCH;
   const long long n = (long long)d->rows * d->Hq;
+  // A masked score of -inf times 0 would be NaN.  Scores below 2^100 times the least normal number change no weight.
+  const float scale_log2 = fmaxf(d->scale * 1.4426950408889634f, 0x1p-126f);
   int by_shift = 0;
   while (1 << by_shift < group) ++by_shift;
-  const PrParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, d->scale * 1.4426950408889634f,
+  const PrParams p = {paged_view(d), (const uint16_t*)d->x, d->x_stride_row, d->x_stride_head, (uint16_t*)d->out, scale_log2,
                       group, (uint32_t)(((1ull << (31 + by_shift)) + group - 1) / group), by_shift, pl.tile_rows, pl.box_tokens, pl.tiles, pl.splits,
                       (float*)d->workspace, (float2*)((float*)d->workspace + pl.splits * n * D)};
   if (launch_pdl<true>(kern, dim3((unsigned)pl.items), dim3(PR_THREADS), Cfg::SMEM_BYTES, stream, tq, tk, tv, p) != cudaSuccess)

@@ -176,8 +176,8 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
     rows, n_heads, D = q.shape
     native = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 <= scale < math.inf:
-        raise ValueError(f"{what}: scale must be finite and not negative, got {scale}")
+    if not 0.0 <= scale <= 1e38:
+        raise ValueError(f"{what}: scale must lie in [0, 1e38], got {scale}")
     if not native:
         return _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale)
     if q.get_device() != nat.device_index():

@@ -294,6 +294,16 @@ def test_strided_queries_and_other_scales():
     _check_attention(q, k, v, wide, lens)
 
 
+@pytest.mark.parametrize("scale", [0.0, 1e-42, 1e-3, 2.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scales(scale, D):
+    """Scale 0, or one that 32 bits flush to 0, weighs all keys alike, those behind a row's last one not at all."""
+    new, past = [200, 1, 0, 3], [100, 0, 7, 500]
+    k, v, table, lens = make_cache([a + b for a, b in zip(new, past)], 2, 32, D, torch.bfloat16, "cuda")
+    _check_attention(_randn(204, 6, D, dtype=torch.bfloat16), k, v, table, lens, _i32(0, 200, 201, 201, 204), scale=scale)
+    _check_attention(_randn(4, 6, D, dtype=torch.bfloat16), k, v, table, lens, scale=scale)
+
+
 @pytest.mark.parametrize("hq,hkv,D", [(128, 1, 64), (100, 1, 128), (66, 2, 64)])
 def test_widest_groups(hq, hkv, D):
     """A query tile of one token; groups that fill it, or not."""
