@@ -1,4 +1,6 @@
 """Paged key-value cache on the GPU: every operator against its definition in 64 bits, alone and as a model uses them."""
+import threading
+
 import pytest
 import torch
 
@@ -534,6 +536,61 @@ def test_captured_step_follows_its_tables():
         _status()       # idle slots have a row each by the prompt's offsets, more rows than tokens
     except Exception:
         pass
+
+
+def _two_batches():
+    """Calls of decode and prompt attention over two caches, all with parts to join, and the results each gives alone."""
+    F = _F()
+    calls = []
+    for seed, (hq, hkv, D) in enumerate([(24, 8, 128), (32, 4, 64)]):
+        k, v, table, lens = make_cache([9000, 30, 0, 4000], hkv, 64, D, torch.bfloat16, "cuda", seed=seed)
+        one, many = _randn(4, hq, D, dtype=torch.bfloat16, seed=seed), _randn(43, hq, D, dtype=torch.bfloat16, seed=seed + 2)
+        offsets = _i32(0, 20, 23, 23, 43)
+        calls.append(lambda a=(one, k, v, table, lens): F.decode_attention(*a))
+        calls.append(lambda a=(many, k, v, table, lens, offsets): F.prompt_attention(*a))
+    return calls, [c() for c in calls]
+
+
+def test_streams_and_threads_side_by_side():
+    calls, alone = _two_batches()
+    torch.cuda.synchronize()
+    results = [[] for _ in calls]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                results[i].append(calls[i]())
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, got in enumerate(results):
+        assert len(got) == 30 and all(_same(x, alone[i]) for x in got)
+    _status()
+
+
+def test_captured_graphs_side_by_side():
+    """Graphs of the same calls replayed at the same time on two streams have workspaces of their own."""
+    calls, alone = _two_batches()
+    graphs = []
+    for order in (calls, calls[::-1]):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [c() for c in order]
+        graphs.append((graph, outs, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, outs, _), want in zip(graphs, (alone, alone[::-1])):
+        assert all(_same(x, y) for x, y in zip(outs, want))
+    _status()
 
 
 @pytest.mark.parametrize("kind", ["llama", "gpt2"])
