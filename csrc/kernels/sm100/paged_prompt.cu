@@ -281,8 +281,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           // the host splits by what the table holds; at least three tiles a split are worth it
           const int most = max(n[0], n[1]), splits = min(p.splits, max(1, most / 3)), mine = min(it.split, splits);
           it.direct = splits == 1;
-          it.lo = (int)((long long)most * mine / splits);
-          const int hi = (int)((long long)most * min(mine + 1, splits) / splits);
+          it.lo = splits == 1 ? most * mine : (unsigned)(most * mine) / splits;
+          const int hi = splits == 1 ? most : (unsigned)(most * min(mine + 1, splits)) / splits;   // (32 splits of 2^23 tiles at most)
           it.hi[0] = min(hi, n[0]);
           it.hi[1] = min(hi, n[1]);
         }
