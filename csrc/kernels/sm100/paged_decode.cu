@@ -85,9 +85,6 @@ __device__ __forceinline__ void load16(uint32_t (&w)[4], const uint16_t* p, bool
       : "l"(p), "r"((int)there));
 }
 
-// First unit of CTA i of n over `units` units
-__device__ __forceinline__ int dec_start(int units, int i, int n) { return (int)((long long)units * i / n); }
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) decode_attention_kernel(const DecParams p) {
   using Cfg = DecCfg<D, NT>;
@@ -140,8 +137,10 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
     if (threadIdx.x == 0 && p.open) p.open[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-  int u = dec_start(units, blockIdx.x, ctas);
-  const int u_end = dec_start(units, blockIdx.x + 1, ctas);
+  const unsigned each = (unsigned)units / ctas, left_over = units - each * ctas;
+  auto start = [&](int i) { return (int)(each * i + left_over * i / (unsigned)ctas); };   // first unit of CTA i: units i / ctas
+  int u = start(blockIdx.x);
+  const int u_end = start(blockIdx.x + 1);
   int4 opened = make_int4(-1, 0, 0, 0);
   int b;   // the sequence of unit u
   {
@@ -274,8 +273,11 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         }
       }
       if (done_t0 <= extra && !whole) {
-        const long long behind = (long long)before[done_b] * head_blocks + (done_hb + 1) * done_units;   // the pair's last unit + 1
-        opened = make_int4(done_b, done_hb, (int)((behind * ctas - 1) / units), 0);
+        const int last = before[done_b] * head_blocks + (done_hb + 1) * done_units - 1;   // unit of the pair
+        int cta = (int)((float)last * ctas / units);
+        while (start(cta) > last) --cta;
+        while (start(cta + 1) <= last) ++cta;
+        opened = make_int4(done_b, done_hb, cta, 0);
       }
       if (!live) break;
       __syncthreads();
