@@ -21,7 +21,7 @@
 // and a captured launch stays balanced whatever its lengths become.
 //
 // Bytes of the cache a second, of a measured copy's 6.47 TB/s: 128 sequences of up to 8192 tokens, 24 / 8 heads of 128, 334 us,
-// 6.7 TB/s; one of 131071, 88.7 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 87.6 us, 6.1; 64 of them 26.4 us, 4.6.  What is left
+// 6.7 TB/s; one of 131071, 88.7 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 87.6 us, 6.1; 64 of them 26.1 us, 4.7.  What is left
 // is a chain at both ends: lengths, page numbers, first keys (4 us from the launch to the first product), and 3 us for the join.
 #include "paged.cuh"
 

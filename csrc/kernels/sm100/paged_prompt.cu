@@ -24,7 +24,7 @@
 // - A CTA takes the next item when it has done its own (clusterlaunchcontrol: it takes over a CTA of the grid that has not
 //   started).  Dealt out in advance, 16 runs of 8000 tokens in all took 119 us in place of 102, 32 / 4 heads of 64.
 //
-// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 326 us, 1.26 PFLOP/s, in short bursts, more for seconds
+// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 324 us, 1.27 PFLOP/s, in short bursts, more for seconds
 // under the power cap (990 W; the dense kernel 317 and 368); 16 runs of 8000 in all, 32 / 4 heads of 64, 105 us, 0.50 (1965 MHz,
 // 840 W); 256 tokens behind 32768, 24 / 8 heads of 128, 99 us, 1.04; 37 tokens 7 us.
 // What bounds it: a K / V tile takes a pair of query tiles 1.5 to 1.6 us at either head_dim, of which the tensor pipe, the
@@ -34,7 +34,10 @@
 // scheduler taking turns with theirs (331 -> 393 us at head_dim 64); P in columns of its own at head_dim 64 and the next scores
 // ahead of the product (331 -> 410); three regions for scores there, in turn, with the same aim (346 -> 361); masked tiles
 // without the products and exponentials of keys that no row sees (102 -> 118); an eighth of the exponentials by a polynomial on the
-// multiply-add units (326 -> 337, a quarter 342).
+// multiply-add units (326 -> 337, a quarter 342); the first scores of the next item between the last products of this one's tiles
+// (104 -> 108); rows written as whole lines by four lanes each (nothing, without the cost of the exchange).
+// 16 runs of 8000 in all: outside its tiles an item takes 4000 clocks, 16 % of the time (next item 800, first scores 1000, last product
+// 350, epilogue 1700; head_dim 128: epilogue 3000, 6000 where it leaves fp32 parts).
 // Without any maximum, as a limit, 1 % is gained.
 #include "paged.cuh"
 
