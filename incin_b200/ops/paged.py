@@ -53,9 +53,9 @@ def _int_row(what: str, name: str, t, last: int) -> None:
         raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
 
 
-def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int) -> bool:
-    """Whether the kernels take the call (else the CPU does), once everything about the arguments is in order.  These checks
-    are a good part of a short call's time: no attribute is asked for twice."""
+def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int):
+    """The device's index (-1: the CPU does the call) and what ``_launch`` wants to know of the shapes, once everything about
+    the arguments is in order.  These checks are a good part of a short call's time: no attribute is asked for twice."""
     shape, dtype = k_pages.shape, x.dtype
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages must both be [pages, kv_heads, page_size, head_dim], got "
@@ -88,13 +88,14 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
             raise ValueError(f"{what}: offsets on {offsets.device}, the others on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    dims = (width, seqs, rows, pages, size, n_heads, hkv, D)
     if at < 0:
-        return False
+        return at, dims
     if dtype not in _KIND or D not in (64, 128):
         raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
     if n_heads // hkv > 128:
         raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
-    return True
+    return at, dims
 
 
 def _page_strides(what: str, name: str, t, at: int) -> tuple[int, int, int]:
@@ -104,13 +105,12 @@ def _page_strides(what: str, name: str, t, at: int) -> tuple[int, int, int]:
     return a, b, c
 
 
-def _launch(fn, what: str, x, x_strides, k_pages, v_pages, table, lengths, offsets, n_heads: int, out, scale: float = 0.0, args=(), workspace=None):
-    pages, hkv, size, D = k_pages.shape
-    seqs, width = table.shape
+def _launch(fn, what: str, dims, x, x_at: int, x_row: int, x_head: int, k_pages, v_pages, table, lengths, offsets, out, scale: float = 0.0,
+            args=(), workspace=None):
     k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
     fields = (k_at, v_at, *_page_strides(what, "k_pages", k_pages, k_at), *_page_strides(what, "v_pages", v_pages, v_at), table.data_ptr(),
-              table.stride(0), lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), width, seqs, x.shape[0], pages, size,
-              n_heads, hkv, D, _KIND[x.dtype], scale, x.data_ptr(), *x_strides, out.data_ptr())
+              table.stride(0), lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), *dims, _KIND[x.dtype], scale, x_at, x_row,
+              x_head, out.data_ptr())
     status = status_word(x.device).data_ptr()
     desc, room = _pack_desc(*fields, 0, status), None
     if workspace is not None:
@@ -138,18 +138,20 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
         raise ValueError(f"kv_append: rows of {wide} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
     if theta is not None and not 1.0 <= theta < 1e300:
         raise ValueError(f"kv_append: theta must be at least 1, got {theta}")
-    if not _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads):
+    at, dims = _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    if at < 0:
         return _append_cpu(qkv.unflatten(1, (n_heads + 2 * hkv, D)), k_pages, v_pages, table, lengths, offsets, n_heads, theta)
-    if qkv.get_device() != nat.device_index():
+    if at != nat.device_index():
         with torch.cuda.device(qkv.device):
             return kv_append(qkv, k_pages, v_pages, table, lengths, offsets, n_heads=n_heads, theta=theta)
     q = qkv.new_empty((rows, n_heads, D))
     if rows == 0:
         return q
-    step, one = qkv.stride()
-    if one != 1 or step % 8 or step <= 0 or qkv.data_ptr() % 16:   # the kernel wants dense heads on 16-byte boundaries
+    (step, one), x_at = qkv.stride(), qkv.data_ptr()
+    if one != 1 or step % 8 or step <= 0 or x_at % 16:   # the kernel wants dense heads on 16-byte boundaries
         qkv, step = qkv.clone(memory_format=torch.contiguous_format), wide
-    return _launch(nat.cuda().incin_kv_append, "kv_append", qkv, (step, D), k_pages, v_pages, table, lengths, offsets, n_heads, q,
+        x_at = qkv.data_ptr()
+    return _launch(nat.cuda().incin_kv_append, "kv_append", dims, qkv, x_at, step, D, k_pages, v_pages, table, lengths, offsets, q,
                    args=(theta or 0.0,))
 
 
@@ -170,29 +172,33 @@ def prompt_attention(q, k_pages, v_pages, table, lengths, offsets, *, scale: flo
 
 
 def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
-    if q.dim() != 3 or k_pages.dim() != 4 or q.shape[2] != k_pages.shape[3]:
-        raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(q.shape)} and pages "
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what}: q must be [rows, heads, head_dim], got {tuple(shape)}")
+    rows, n_heads, D = shape
+    at, dims = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    if D != dims[-1]:
+        raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(shape)} and pages "
                          f"{tuple(k_pages.shape)}")
-    rows, n_heads, D = q.shape
-    native = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 <= scale <= 1e38:
         raise ValueError(f"{what}: scale must lie in [0, 1e38], got {scale}")
-    if not native:
+    if at < 0:
         return _attend_cpu(q, k_pages, v_pages, table, lengths, offsets, scale)
-    if q.get_device() != nat.device_index():
+    if at != nat.device_index():
         with torch.cuda.device(q.device):
             return _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale)
     out = q.new_empty((rows, n_heads, D))
     if rows == 0:
         return out
-    a, b, one = q.stride()
-    if one != 1 or (a | b) % 8 or a <= 0 or b <= 0 or q.data_ptr() % 16:   # the kernels want dense heads on 16-byte boundaries
+    (a, b, one), x_at = q.stride(), q.data_ptr()
+    if one != 1 or (a | b) % 8 or a <= 0 or b <= 0 or x_at % 16:   # the kernels want dense heads on 16-byte boundaries
         q, a, b = q.clone(memory_format=torch.contiguous_format), n_heads * D, D
+        x_at = q.data_ptr()
     lib = nat.cuda()
     fn, room = ((lib.incin_decode_attention, lib.incin_decode_attention_workspace) if offsets is None else
                 (lib.incin_prompt_attention, lib.incin_prompt_attention_workspace))
-    return _launch(fn, what, q, (a, b), k_pages, v_pages, table, lengths, offsets, n_heads, out, scale, workspace=room)
+    return _launch(fn, what, dims, q, x_at, a, b, k_pages, v_pages, table, lengths, offsets, out, scale, workspace=room)
 
 
 # -------------------------------------------------------------------------------------------------------------- pages
