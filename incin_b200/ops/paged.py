@@ -209,21 +209,22 @@ def copy_pages(storage, src, dst):
     times; a destination must be named once and be nobody's source (a page may be its own copy).  Pairs that break this, or
     name no page, raise on the CPU; on CUDA they are left out and reported through ``ops.gemm.check_status``, the earliest of
     several equal destinations being kept."""
-    if storage.dim() < 4 or not storage.is_contiguous():
-        raise ValueError(f"copy_pages: storage must be dense [..., pages, kv_heads, page_size, head_dim], got {tuple(storage.shape)}, "
+    shape, pairs, at = storage.shape, src.shape, storage.get_device()
+    if len(shape) < 4 or not storage.is_contiguous():
+        raise ValueError(f"copy_pages: storage must be dense [..., pages, kv_heads, page_size, head_dim], got {tuple(shape)}, "
                          f"strides {storage.stride()}")
-    if src.dim() != 1 or src.shape != dst.shape or src.dtype != torch.int32 or dst.dtype != torch.int32:
+    if len(pairs) != 1 or pairs != dst.shape or src.dtype is not torch.int32 or dst.dtype is not torch.int32:
         raise ValueError(f"copy_pages: src and dst must be int32 [pairs], got {tuple(src.shape)} {src.dtype} and {tuple(dst.shape)} {dst.dtype}")
-    if src.device != storage.device or dst.device != storage.device:
+    if src.get_device() != at or dst.get_device() != at:
         raise ValueError(f"copy_pages: tensors on {storage.device}, {src.device} and {dst.device}")
     if torch.is_grad_enabled() and storage.requires_grad:
         raise RuntimeError("copy_pages has no backward pass: call it under torch.no_grad()")
-    pages = storage.shape[-4]
-    page_bytes = math.prod(storage.shape[-3:]) * storage.element_size()
-    outer = math.prod(storage.shape[:-4])
+    *outer, pages, heads, size, D = shape
+    page_bytes = heads * size * D * storage.element_size()
+    outer = math.prod(outer)
     if page_bytes % 16:
         raise ValueError(f"copy_pages: pages of {page_bytes} bytes, not a multiple of 16")
-    if not storage.is_cuda:
+    if at < 0:
         a, b = src.tolist(), dst.tolist()
         moves = [(i, j) for i, j in zip(a, b) if i != j]
         if any(not 0 <= i < pages for i in a + b):
@@ -234,15 +235,18 @@ def copy_pages(storage, src, dst):
             flat = storage.view(outer, pages, -1)
             flat[:, [j for _, j in moves]] = flat[:, [i for i, _ in moves]]
         return storage
-    if src.numel() == 0 or storage.numel() == 0:
+    n = pairs[0]
+    if n == 0 or page_bytes * pages * outer == 0:
         return storage
-    if storage.data_ptr() % 16:
+    ptr = storage.data_ptr()
+    if ptr % 16:
         raise nat.NativeError("copy_pages: storage must start on a 16-byte boundary")
-    if storage.get_device() != nat.device_index():
+    if at != nat.device_index():
         with torch.cuda.device(storage.device):
             return copy_pages(storage, src, dst)
-    src, dst = src.contiguous(), dst.contiguous()
-    nat.check(nat.cuda().incin_copy_pages(storage.data_ptr(), src.data_ptr(), dst.data_ptr(), src.numel(), outer, pages, page_bytes,
+    if n > 1:
+        src, dst = src.contiguous(), dst.contiguous()
+    nat.check(nat.cuda().incin_copy_pages(ptr, src.data_ptr(), dst.data_ptr(), n, outer, pages, page_bytes,
                                           status_word(storage.device).data_ptr(), nat.stream_ptr()), "copy_pages")
     return storage
 
