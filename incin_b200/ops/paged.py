@@ -48,14 +48,14 @@ _KIND = {torch.bfloat16: nat.GEMM_IN_BF16, torch.float16: nat.GEMM_IN_FP16}
 
 
 # ------------------------------------------------------------------------------------------------------------- checks
-def _int_row(what: str, name: str, t, last: int) -> None:
-    if t.dtype is not torch.int32 or (last > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
+def _not_int_row(what: str, name: str, t):
+    return ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
 
 
 def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int):
-    """The device's index (-1: the CPU does the call) and what ``_launch`` wants to know of the shapes, once everything about
-    the arguments is in order.  These checks are a good part of a short call's time: no attribute is asked for twice."""
+    """The device's index (-1: the CPU does the call), what ``_launch`` wants to know of the shapes and the table's row stride,
+    once everything about the arguments is in order.  These checks are a good part of a short call's time: no attribute is
+    asked for twice."""
     shape, dtype = k_pages.shape, x.dtype
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages must both be [pages, kv_heads, page_size, head_dim], got "
@@ -72,8 +72,11 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
         raise ValueError(f"{what}: table must be [sequences, entries] and lengths [sequences], got {tuple(t_shape)} and "
                          f"{tuple(l_shape)}")
     seqs, width = t_shape
-    _int_row(what, "table", table, width)
-    _int_row(what, "lengths", lengths, seqs)
+    t_row, t_one = table.stride()
+    if table.dtype is not torch.int32 or (width > 1 and t_one != 1):
+        raise _not_int_row(what, "table", table)
+    if lengths.dtype is not torch.int32 or (seqs > 1 and lengths.stride(0) != 1):
+        raise _not_int_row(what, "lengths", lengths)
     at = x.get_device()   # -1 on the CPU
     if k_pages.get_device() != at or v_pages.get_device() != at or table.get_device() != at or lengths.get_device() != at:
         raise ValueError(f"{what}: tensors on {[str(t.device) for t in (x, k_pages, v_pages, table, lengths)]}")
@@ -83,19 +86,21 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
     else:
         if offsets.dim() != 1 or offsets.shape[0] != seqs + 1:
             raise ValueError(f"{what}: offsets must be [sequences + 1] = [{seqs + 1}], got {tuple(offsets.shape)}")
-        _int_row(what, "offsets", offsets, seqs + 1)
+        if offsets.dtype is not torch.int32 or offsets.stride(0) != 1:
+            raise _not_int_row(what, "offsets", offsets)
         if offsets.get_device() != at:
             raise ValueError(f"{what}: offsets on {offsets.device}, the others on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
-    dims = (width, seqs, rows, pages, size, n_heads, hkv, D)
+    kind = _KIND.get(dtype, -1)
+    dims = (width, seqs, rows, pages, size, n_heads, hkv, D, kind)
     if at < 0:
-        return at, dims
-    if dtype not in _KIND or D not in (64, 128):
+        return at, dims, t_row
+    if kind < 0 or (D != 64 and D != 128):
         raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
     if n_heads // hkv > 128:
         raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
-    return at, dims
+    return at, dims, t_row
 
 
 def _page_strides(what: str, name: str, t, at: int) -> tuple[int, int, int]:
@@ -105,12 +110,11 @@ def _page_strides(what: str, name: str, t, at: int) -> tuple[int, int, int]:
     return a, b, c
 
 
-def _launch(fn, what: str, dims, x, x_at: int, x_row: int, x_head: int, k_pages, v_pages, table, lengths, offsets, out, scale: float = 0.0,
-            args=(), workspace=None):
+def _launch(fn, what: str, dims, t_row: int, x, x_at: int, x_row: int, x_head: int, k_pages, v_pages, table, lengths, offsets, out,
+            scale: float = 0.0, args=(), workspace=None):
     k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
     fields = (k_at, v_at, *_page_strides(what, "k_pages", k_pages, k_at), *_page_strides(what, "v_pages", v_pages, v_at), table.data_ptr(),
-              table.stride(0), lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), *dims, _KIND[x.dtype], scale, x_at, x_row,
-              x_head, out.data_ptr())
+              t_row, lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(), *dims, scale, x_at, x_row, x_head, out.data_ptr())
     status = status_word(x.device).data_ptr()
     desc, room = _pack_desc(*fields, 0, status), None
     if workspace is not None:
@@ -138,7 +142,7 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
         raise ValueError(f"kv_append: rows of {wide} elements, not ({n_heads} + 2 * {hkv}) heads of {D}")
     if theta is not None and not 1.0 <= theta < 1e300:
         raise ValueError(f"kv_append: theta must be at least 1, got {theta}")
-    at, dims = _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    at, dims, t_row = _check("kv_append", qkv, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
     if at < 0:
         return _append_cpu(qkv.unflatten(1, (n_heads + 2 * hkv, D)), k_pages, v_pages, table, lengths, offsets, n_heads, theta)
     if at != nat.device_index():
@@ -151,7 +155,7 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
     if one != 1 or step % 8 or step <= 0 or x_at % 16:   # the kernel wants dense heads on 16-byte boundaries
         qkv, step = qkv.clone(memory_format=torch.contiguous_format), wide
         x_at = qkv.data_ptr()
-    return _launch(nat.cuda().incin_kv_append, "kv_append", dims, qkv, x_at, step, D, k_pages, v_pages, table, lengths, offsets, q,
+    return _launch(nat.cuda().incin_kv_append, "kv_append", dims, t_row, qkv, x_at, step, D, k_pages, v_pages, table, lengths, offsets, q,
                    args=(theta or 0.0,))
 
 
@@ -176,8 +180,8 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
     if len(shape) != 3:
         raise ValueError(f"{what}: q must be [rows, heads, head_dim], got {tuple(shape)}")
     rows, n_heads, D = shape
-    at, dims = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
-    if D != dims[-1]:
+    at, dims, t_row = _check(what, q, k_pages, v_pages, table, lengths, offsets, rows, n_heads)
+    if D != dims[7]:
         raise ValueError(f"{what}: q must be [rows, heads, head_dim] of the cache's head_dim, got {tuple(shape)} and pages "
                          f"{tuple(k_pages.shape)}")
     scale = D ** -0.5 if scale is None else float(scale)
@@ -198,7 +202,7 @@ def _attend(what, q, k_pages, v_pages, table, lengths, offsets, scale):
     lib = nat.cuda()
     fn, room = ((lib.incin_decode_attention, lib.incin_decode_attention_workspace) if offsets is None else
                 (lib.incin_prompt_attention, lib.incin_prompt_attention_workspace))
-    return _launch(fn, what, dims, q, x_at, a, b, k_pages, v_pages, table, lengths, offsets, out, scale, workspace=room)
+    return _launch(fn, what, dims, t_row, q, x_at, a, b, k_pages, v_pages, table, lengths, offsets, out, scale, workspace=room)
 
 
 # -------------------------------------------------------------------------------------------------------------- pages
