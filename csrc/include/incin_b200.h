@@ -249,7 +249,7 @@ int incin_flash_attn_bwd(const incin_attn_desc* desc, void* stream);
  * table or an entry outside [0, pages) that is met writes KernelStatus 6 to *status; the entry reads as zeros and is not
  * written through.  Outputs of rows outside every sequence, and of sequences without tokens, are zeros.
  * Hq is a multiple of Hkv, Hq / Hkv at most 128.  A table holds up to 2^30 tokens a sequence; decode wants token strides
- * below 2^23 elements. */
+ * below 2^23 elements.  scale (of attention only) lies in [0, 1e38]. */
 typedef struct incin_paged_desc {
   void *k_pages, *v_pages;
   long long k_stride_page, k_stride_head, k_stride_token;
@@ -265,7 +265,7 @@ typedef struct incin_paged_desc {
   void* workspace; /* 32-byte aligned, as many bytes as the operation's _workspace function says; may be NULL for 0 */
   void* status;
 } incin_paged_desc;
-/* Rotates queries and keys of the new rows to their positions (rotate-half pairs, theta > 0; 0 leaves them as they are),
+/* Rotates queries and keys of the new rows to their positions (rotate-half pairs, theta at least 1; 0 leaves them as they are),
  * writes keys and values into the cache and the queries to out. */
 int incin_kv_append(const incin_paged_desc* desc, double theta, void* stream);
 /* Attention of one new token per sequence (offsets unused, rows == seqs) over its cached tokens. */

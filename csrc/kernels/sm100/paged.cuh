@@ -39,12 +39,16 @@ inline int check_paged(const incin_paged_desc* d) {
   if (((uintptr_t)d->k_pages | (uintptr_t)d->v_pages | (uintptr_t)d->x | (uintptr_t)d->out) & 15 || ((uintptr_t)d->workspace & 31))
     return INCIN_ERR_ALIGNMENT;
   if ((long long)d->table_width * d->page_size > (1ll << 30)) return INCIN_ERR_TOO_LARGE;   // positions are counted in 32 bits
-  if (!(d->scale >= 0.f && d->scale <= 1e38f)) return INCIN_ERR_ARGUMENT;   // times log2(e) in 32 bits
   const long long strides[] = {d->k_stride_page, d->k_stride_head, d->k_stride_token, d->v_stride_page, d->v_stride_head,
                                d->v_stride_token, d->x_stride_row, d->x_stride_head};
   for (long long s : strides)
     if (s % 8) return INCIN_ERR_ALIGNMENT;
   return INCIN_OK;
+}
+// ... and attention besides.
+inline int check_paged_attention(const incin_paged_desc* d) {
+  const int rc = check_paged(d);
+  return rc || (d->scale >= 0.f && d->scale <= 1e38f) ? rc : INCIN_ERR_ARGUMENT;   // times log2(e) in 32 bits
 }
 
 __device__ __forceinline__ void flag_bad_index(int* status) {

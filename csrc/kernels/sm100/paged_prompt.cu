@@ -826,7 +826,7 @@ extern "C" long long incin_prompt_attention_workspace(const incin_paged_desc* d)
 
 extern "C" int incin_prompt_attention(const incin_paged_desc* d, void* stream) {
   using namespace incin;
-  const int rc = check_paged(d);
+  const int rc = check_paged_attention(d);
   if (rc) return rc;
   if (!d->offsets) return INCIN_ERR_ARGUMENT;
   const cudaStream_t s = (cudaStream_t)stream;
