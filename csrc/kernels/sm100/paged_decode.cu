@@ -1,6 +1,6 @@
 // Attention of one new token per sequence over a paged key-value cache.
 //
-//   o_h = sum_j p_hj v_j,  p_hj = 2^(z_hj - m_h) / l_h,  z = scale log2(e) q_h k_j,  j < lengths[b]
+//   o_h = sum_j p_hj v_j,  p_hj = 2^(c (z_hj - m_h)) / l_h,  z = q_h k_j,  c = scale log2(e),  j < lengths[b]
 //
 // Every cached key and value is used once, so the bytes of the cache bound it.  The query heads of a key head are the
 // columns of one product: S^T [16 keys x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T with m16n8k16 matrix
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
 #pragma unroll
         for (int w = 0; w < DEC_WARPS; ++w) {
           // a warp without keys has m = -inf, l = 0 and O = 0
-          const float f = sm_m[w][h] == top ? 1.f : exp2f(sm_m[w][h] - top);
+          const float f = sm_m[w][h] == top ? 1.f : exp2f((sm_m[w][h] - top) * p.scale_log2);
           sum += f * sm_l[w][h];
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] += f * sm_o[w][h][d + e];
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           mma16816<T>(odd, kr[0][j][2], kr[1][j][2], kr[0][j][3], kr[1][j][3], q[t][j][2], q[t][j][3]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = (even[e] + odd[e]) * p.scale_log2;
+        for (int e = 0; e < 4; ++e) s[t][e] = even[e] + odd[e];
       }
       if (next < key_end) load_k(next, step);
       // element e of s: key r (+ 8 from e = 2 on), head 2 q4 + (e & 1)
@@ -336,19 +336,19 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           for (int e = 0; e < 4; ++e)
             if (key + r + (e >> 1) * 8 >= key_end) s[t][e] = -CUDART_INF_F;
       }
-      // The reference of the exponentials moves only when the maximum has grown by more than 2^8; O and l are divided by
-      // each other in the end.
+      // The reference m of the exponentials moves only when the maximum has grown by more than 2^8; O and l are divided by
+      // each other in the end.  m is a score before its scale: the difference is exactly 0 at the maximum, whatever the scale.
       uint32_t pb[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float mx[2] = {fmaxf(s[t][0], s[t][2]), fmaxf(s[t][1], s[t][3])};
-        if (__any_sync(0xffffffffu, mx[0] > m[t][0] + 8.f || mx[1] > m[t][1] + 8.f)) {
+        if (__any_sync(0xffffffffu, (mx[0] - m[t][0]) * p.scale_log2 > 8.f || (mx[1] - m[t][1]) * p.scale_log2 > 8.f)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
-            const bool move = mx[e] > m[t][e] + 8.f;
-            const float alpha = move ? exp2f(m[t][e] - mx[e]) : 1.f;
+            const bool move = (mx[e] - m[t][e]) * p.scale_log2 > 8.f;
+            const float alpha = move ? exp2f((m[t][e] - mx[e]) * p.scale_log2) : 1.f;
             if (move) m[t][e] = mx[e];
             l[t][e] *= alpha;
 #pragma unroll
@@ -361,12 +361,18 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           }
         }
         const float r0 = m[t][0] == -CUDART_INF_F ? 0.f : m[t][0], r1 = m[t][1] == -CUDART_INF_F ? 0.f : m[t][1];
-        const float p0 = exp2f(s[t][0] - r0), p1 = exp2f(s[t][1] - r1), p2 = exp2f(s[t][2] - r0), p3 = exp2f(s[t][3] - r1);
-        l[t][0] += p0 + p2;
-        l[t][1] += p1 + p3;
+        float w[4] = {exp2f((s[t][0] - r0) * p.scale_log2), exp2f((s[t][1] - r1) * p.scale_log2), exp2f((s[t][2] - r0) * p.scale_log2),
+                      exp2f((s[t][3] - r1) * p.scale_log2)};
+        if (key + 16 > key_end) {   // (-inf times a scale of 0 is no number)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key + r + (e >> 1) * 8 >= key_end) w[e] = 0.f;
+        }
+        l[t][0] += w[0] + w[2];
+        l[t][1] += w[1] + w[3];
         // P in the cache's type, as the instruction wants it: half a step of relative error a weight
-        pb[t][0] = transpose8x8(T::pack(p0, p1));
-        pb[t][1] = transpose8x8(T::pack(p2, p3));
+        pb[t][0] = transpose8x8(T::pack(w[0], w[1]));
+        pb[t][1] = transpose8x8(T::pack(w[2], w[3]));
       }
 #pragma unroll
       for (int j = 0; j < VJ; ++j)
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) decode_join_kernel(const DecPara
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
   auto add = [&](const Part& a) {
-    const float f = a.m == top ? 1.f : exp2f(a.m - top);
+    const float f = a.m == top ? 1.f : exp2f((a.m - top) * p.scale_log2);
     sum += f * a.l;
     acc = make_float4(acc.x + f * a.o.x, acc.y + f * a.o.y, acc.z + f * a.o.z, acc.w + f * a.o.w);
   };

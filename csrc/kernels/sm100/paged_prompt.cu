@@ -56,6 +56,7 @@ constexpr int PR_THREADS = 384;   // warp 0: items and TMA, 1: tcgen05 issue, 2-
 // sequences spills, 8 runs of 8000 in all, 12 heads of 64, 57.5 us in place of 54.8; 120 and 192: 57.9.)
 constexpr int PR_REGS_ISSUE = 104, PR_REGS_SOFTMAX = 200;
 constexpr int PR_ITEMS = 3;       // slots of the item ring
+constexpr float PR_FAR = 64.f;    // references past this, times scale log2(e), are taken off the scores in an instruction of their own
 
 template <int D>
 struct PrCfg {
@@ -557,7 +558,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const bool live_row = w < p.tiles && row < p.tile_rows && mine < it.tokens;
       const int limit = it.pos0 + (live_row ? mine : min(first_token, it.tokens - 1));   // the last key that the row sees
       const int all_see = it.pos0 + first_token;                 // ... and the last one that every row of the tile sees
-      float m_ref = -CUDART_INF_F;
+      float m_ref = -CUDART_INF_F;   // a score before its scale
+      float bias = 0.f;              // -scale m_ref, or 0 where it is taken off the scores themselves
+      bool far = false;              // ... which the whole warp does when the reference of one of its rows is far from 0
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = lo; j < hi; ++j) {
         if (!mbar_wait(&s_full[w], s_phase, abort_flag, c.status, kStatusTimeoutTmemFull)) { ok = false; break; }
@@ -579,18 +582,30 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int e = 0; e < PR_BM; e += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(fmaxf(mx4[k], __uint_as_float(s[e + k * 2])), __uint_as_float(s[e + k * 2 + 1]));
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-        // lazy rescale: only move the reference when the maximum grew by more than 2^8
-        const bool need = mx > m_ref + 8.0f;
-        if (__any_sync(0xffffffffu, need)) {
-          const float alpha = need ? exp2f(m_ref - mx) : 1.0f;   // 0 the first time
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        // lazy rescale: only move the reference when the maximum grew by more than 2^8.  P = exp2(scale (s - m_ref)) as one
+        // instruction, scale s - scale m_ref, is off by half a step of the rounded product, 2^-18 at most below PR_FAR;
+        // past it, where it could be any power of 2, the difference comes first.  (16 runs of 8000 in all, 32 / 4
+        // heads of 64: 104.6 us without it, 107.0 as it is; 113 with far references in a branch of their own in front of the
+        // exponentials, 111 with scale times difference everywhere, 107.5 with the differences taken in tensor memory.)
+        const bool need = (mx - m_ref) * p.scale_log2 > 8.0f, moves = __any_sync(0xffffffffu, need);
+        if (moves || far) {
+          const float alpha = need ? exp2f((m_ref - mx) * p.scale_log2) : 1.0f;   // 0 the first time
           if (need) m_ref = mx;
+          const float ref = m_ref == -CUDART_INF_F ? 0.f : m_ref;   // a row that has only seen scores of -inf weighs them 0
+          // (rows that hold no query have no say: what is in them changes from call to call)
+          far = __any_sync(0xffffffffu, live_row && !(fabsf(ref * p.scale_log2) <= PR_FAR));
+          bias = far ? 0.f : -ref * p.scale_log2;
+          if (far) {
+#pragma unroll
+            for (int e = 0; e < PR_BM; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) - ref);
+          }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             l2[e].x *= alpha;
             l2[e].y *= alpha;
           }
-          if (j > lo) {   // s_full covers O_w += P_w(j-1) V_{j-1}: O_w is at rest
+          if (j > lo && moves) {   // s_full covers O_w += P_w(j-1) V_{j-1}: O_w is at rest
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
               uint32_t o[32];
@@ -602,10 +617,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
           }
         }
-        // P = exp2(s * scale - m_ref) in the cache's type over the first half of S_w's columns, row sums in fp32; a row that
-        // has only seen scores of -inf weighs them 0
-        const float ref = m_ref == -CUDART_INF_F ? 0.f : -m_ref;
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(ref, ref);
+        // P in the cache's type over the first half of S_w's columns, row sums in fp32
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(bias, bias);
 #pragma unroll
         for (int ch = 0; ch < PR_BM / 32; ++ch) {
           uint32_t pk[16];
@@ -720,7 +733,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
   float top = ml.x;
 #pragma unroll
   for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-  const float weight = ml.x == -CUDART_INF_F ? 0.f : ml.x == top ? 1.f : exp2f(ml.x - top);
+  const float weight = ml.x == -CUDART_INF_F ? 0.f : ml.x == top ? 1.f : exp2f((ml.x - top) * p.scale_log2);
   if (__any_sync(0xffffffffu, ml.y == -2.f)) return;
   const bool nowhere = __any_sync(0xffffffffu, ml.y < 0.f);
   float sum = weight * ml.y, acc[PER] = {};

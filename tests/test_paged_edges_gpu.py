@@ -1,0 +1,66 @@
+"""Paged key-value cache on the GPU where values, arguments or calls are extreme: against definitions in 64 bits."""
+import pytest
+import torch
+
+from _paged import make_cache, tokens_of
+
+pytestmark = pytest.mark.gpu
+
+
+def _F():
+    from incin_b200.ops import functional as F
+    return F
+
+
+def _code():
+    """The status word, cleared: 0, 6 for an index outside its tensors, 1 to 5 for a wait that ran out."""
+    from incin_b200.ops import gemm as G
+    word = G.status_word(torch.device("cuda", torch.cuda.current_device()))
+    code = int(word.item())
+    word.zero_()
+    return code
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _randn(*shape, dtype, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def _reference(q, k, v, table, lengths, offsets, scale):
+    """Softmax over the visible tokens in 64 bits and the weights' sum of |v|, ``[rows, heads, D]`` each."""
+    hq, hkv = q.shape[1], k.shape[1]
+    out, spread = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    for s, n in enumerate(lengths.tolist()):
+        a, b = int(offsets[s]), int(offsets[s + 1])
+        kk, vv = (tokens_of(t, table, s, n).repeat_interleave(hq // hkv, 0) for t in (k, v))
+        seen = torch.arange(n, device="cuda")[None] <= torch.arange(n - (b - a), n, device="cuda")[:, None]
+        p = torch.softmax((q[a:b].double().transpose(0, 1) @ kk.mT * scale).masked_fill(~seen, float("-inf")), -1)
+        out[a:b], spread[a:b] = (p @ vv).transpose(0, 1), (p @ vv.abs()).transpose(0, 1)
+    return out, spread
+
+
+@pytest.mark.parametrize("scale,factor", [(1e4, 1), (1e8, 1), (1e10, 1), (1e12, 1), (1e30, 1), (1e38, 1), (None, 512)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,D", [(6, 2, 64), (24, 8, 128)])
+def test_large_scales(scale, factor, dtype, hq, hkv, D):
+    """Scores are whole numbers, so that 32 bits hold them exactly and other scores than the largest weigh exp(-1e4) or less: the
+    rows are means over the largest scores' values.  Keys of one CTA, split keys, single tokens; a large scale, or large queries
+    and keys."""
+    g = torch.Generator().manual_seed(D)
+    for new, past in (([200, 1, 3], [100, 0, 500]), ([70], [9000])):
+        k, v, table, lens = make_cache([a + b for a, b in zip(new, past)], hkv, 32, D, dtype, "cuda", poison=False)
+        k.copy_(torch.randint(-8, 9, k.shape, generator=g).to(dtype) * factor)
+        q = torch.randint(-8, 9, (sum(new), hq, D), generator=g).to(dtype).cuda() * factor
+        offsets = _i32(0, *torch.tensor(new).cumsum(0).tolist())
+        ones = torch.arange(len(new) + 1)
+        for x, offs, call in ((q, offsets, lambda: _F().prompt_attention(q, k, v, table, lens, offsets, scale=scale)),
+                              (q[:len(new)], ones, lambda: _F().decode_attention(q[:len(new)], k, v, table, lens, scale=scale))):
+            want, spread = _reference(x, k, v, table, lens, offs, D ** -0.5 if scale is None else scale)
+            # equal weights of 1 (or a power of two), sums of a few values in 32 bits, one rounding
+            bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -20 * spread + 2.0 ** -25
+            got = call().double()
+            assert _code() == 0
+            assert ((got - want).abs() <= bound).all(), f"{(got.isnan()).sum().item()} NaN of {got.numel()}"
