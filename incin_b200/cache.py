@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import heapq
 from collections import Counter
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 
 import torch
@@ -54,6 +55,7 @@ class PagedBatch:
         self.lengths = flat[S * width:S * width + S]
         self.offsets = flat[S * width + S:]
         self.single = all(n == 1 for n in counts)
+        self._undo: list[tuple] = []     # what PagedCache.take_back needs
 
     def positions(self) -> torch.Tensor:
         """Positions of the new tokens, ``[rows]`` int64."""
@@ -164,7 +166,8 @@ class PagedCache:
     def extend(self, seqs: list[int], counts: list[int] | None = None) -> PagedBatch:
         """Make room for ``counts[i]`` (default 1) new tokens of each sequence and describe the batch to the operators.
         A shared open page that is about to be written is copied first (all layers and all such pages in one launch).
-        Raises :class:`CacheFull`, with nothing changed, when there are too few free pages."""
+        Raises :class:`CacheFull` when there are too few free pages; whatever it raises, nothing was changed.  The new tokens
+        count as cached from here on: if what should write them fails, :meth:`take_back` the batch."""
         counts = [1] * len(seqs) if counts is None else [int(n) for n in counts]
         if not seqs or len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or min(counts) < 0:
             raise ValueError(f"extend: sequences must be distinct, with one count >= 0 each, got {seqs} and {counts}")
@@ -182,19 +185,43 @@ class PagedCache:
             split.append(shared)
         if need > len(self._free):
             raise CacheFull(f"{need} pages wanted, {len(self._free)} free of {self.n_pages}")
-        src, dst = [], []
-        for s, n, copy in zip(held, counts, split):
-            if copy:
-                old, s.pages[-1] = s.pages[-1], self._take()
-                self._refs[old] -= 1      # its other owners keep it
-                src.append(old)
-                dst.append(s.pages[-1])
-            s.length += n
-            while len(s.pages) * size < s.length:
-                s.pages.append(self._take())
-        if src:
-            self._copy(src, dst)
-        return PagedBatch(self, [s.pages for s in held], [s.length for s in held], counts)
+        src, dst, undo = [], [], []
+        try:
+            for s, n, copy in zip(held, counts, split):
+                undo.append((s, s.length, len(s.pages), s.pages[-1] if copy else None))
+                if copy:
+                    old, s.pages[-1] = s.pages[-1], self._take()
+                    self._refs[old] -= 1      # its other owners keep it
+                    src.append(old)
+                    dst.append(s.pages[-1])
+                s.length += n
+                while len(s.pages) * size < s.length:
+                    s.pages.append(self._take())
+            if src:
+                self._copy(src, dst)
+            batch = PagedBatch(self, [s.pages for s in held], [s.length for s in held], counts)
+        except BaseException:
+            self._restore(undo)
+            raise
+        batch._undo = undo
+        return batch
+
+    def _restore(self, undo: list[tuple]) -> None:
+        while undo:
+            s, length, pages, copied = undo.pop()
+            for p in s.pages[pages:]:
+                self._drop(p)
+            del s.pages[pages:]
+            if copied is not None and s.pages[-1] != copied:
+                self._drop(s.pages[-1])
+                s.pages[-1] = copied
+                self._refs[copied] += 1
+            s.length = length
+
+    def take_back(self, batch: PagedBatch) -> None:
+        """Undo the :meth:`extend` that made ``batch``: lengths, pages and their owners are as before it.  For a pass that failed,
+        before anything else is done with its sequences."""
+        self._restore(batch._undo)
 
     def admit(self, tokens: torch.Tensor, seqs: list[int], counts: list[int] | None, max_seq: int) -> PagedBatch:
         """:meth:`extend` for a model's forward pass: ``tokens`` are the new tokens, no sequence may pass ``max_seq`` and
@@ -206,6 +233,16 @@ class PagedCache:
             if n < 1 or self.length(s) + n > max_seq:
                 raise ValueError(f"sequence {s}: {n} new tokens after {self.length(s)}, the model holds {max_seq}")
         return self.extend(seqs, counts)
+
+    @contextmanager
+    def step(self, tokens: torch.Tensor, seqs: list[int], counts: list[int] | None, max_seq: int):
+        """The batch of :meth:`admit` for a ``with`` block that runs the forward pass; an exception in it takes the tokens back."""
+        batch = self.admit(tokens, seqs, counts, max_seq)
+        try:
+            yield batch
+        except BaseException:
+            self.take_back(batch)
+            raise
 
     # ------------------------------------------------------------------------------------------------ pages
     def _copy(self, src: list[int], dst: list[int]) -> None:

@@ -143,9 +143,9 @@ class GPT2(nn.Module):
         """Append new tokens to cached sequences and return the logits ``[len(seqs), vocab]`` of each one's last token (see
         :meth:`incin_b200.models.llama.Llama.extend`)."""
         cfg = self.cfg
-        batch = cache.admit(tokens, seqs, counts, cfg.max_seq)
-        x = F.embedding(tokens[None], self.wte) + F.embedding(batch.positions()[None], self.wpe)
-        for i, b in enumerate(self.blocks):
-            x = b.extend(x, batch, i)
-        h = F.layer_norm(x[0, batch.last_rows()], self.lnf_g, self.lnf_b, cfg.ln_eps)
-        return F.linear(h, self.wte)[..., : cfg.vocab_size]
+        with cache.step(tokens, seqs, counts, cfg.max_seq) as batch:
+            x = F.embedding(tokens[None], self.wte) + F.embedding(batch.positions()[None], self.wpe)
+            for i, b in enumerate(self.blocks):
+                x = b.extend(x, batch, i)
+            h = F.layer_norm(x[0, batch.last_rows()], self.lnf_g, self.lnf_b, cfg.ln_eps)
+            return F.linear(h, self.wte)[..., : cfg.vocab_size]

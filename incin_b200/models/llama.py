@@ -131,10 +131,10 @@ class Llama(nn.Module):
     def extend(self, tokens, cache, seqs, counts=None):
         """Append new tokens to cached sequences and return the logits ``[len(seqs), vocab]`` of each one's last token.
         ``tokens`` ``[rows]``: ``counts[i]`` (default 1, at least 1) tokens of sequence ``seqs[i]`` of ``cache``
-        (:class:`~incin_b200.cache.PagedCache`), sequence after sequence."""
-        batch = cache.admit(tokens, seqs, counts, self.cfg.max_seq)
-        x = F.embedding(tokens[None], self.embed, None)
-        for i, b in enumerate(self.blocks):
-            x = b.extend(x, batch, i)
-        h = F.rms_norm(x[0, batch.last_rows()], self.final_norm, self.cfg.rms_eps)
-        return F.linear(h, self.lm_head)
+        (:class:`~incin_b200.cache.PagedCache`), sequence after sequence.  A call that raises leaves the cache as it was."""
+        with cache.step(tokens, seqs, counts, self.cfg.max_seq) as batch:
+            x = F.embedding(tokens[None], self.embed, None)
+            for i, b in enumerate(self.blocks):
+                x = b.extend(x, batch, i)
+            h = F.rms_norm(x[0, batch.last_rows()], self.final_norm, self.cfg.rms_eps)
+            return F.linear(h, self.lm_head)

@@ -1,0 +1,77 @@
+"""Paged key-value cache on the CPU: steps that fail, and arguments at the edge of what the operators take."""
+import pytest
+import torch
+
+from incin_b200.cache import PagedCache
+from incin_b200.ops import functional as F
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _model(kind):
+    from incin_b200.models.gpt2 import GPT2, GPT2Config
+    from incin_b200.models.llama import Llama, LlamaConfig
+    return Llama(LlamaConfig.tiny(), seed=1) if kind == "llama" else GPT2(GPT2Config.tiny(), seed=1)
+
+
+def _books(c, seqs):
+    return [(c.length(s), c.pages_of(s)) for s in seqs], list(c._refs), sorted(c._free)
+
+
+class Stop(BaseException):
+    pass
+
+
+@pytest.mark.parametrize("kind", ["llama", "gpt2"])
+@pytest.mark.parametrize("where", ["token", "first layer", "last layer", "interrupt", "copy", "batch"])
+def test_a_failed_step_is_taken_back(kind, where, monkeypatch):
+    """Whatever raises inside a step, lengths, pages and their owners are as before, those of forked sequences too, and the next
+    step gives the logits of the whole text."""
+    import incin_b200.cache as cache_module
+    model = _model(kind)
+    tok = torch.randint(0, 500, (60,), generator=torch.Generator().manual_seed(2))
+    with torch.no_grad():
+        full = model(tok[None])[0]
+    c = PagedCache.of(model, pages=12, page_size=16)
+    a = c.new()
+    model.extend(tok[:30], c, [a], [30])
+    b = c.fork(a)                        # an open page of two owners
+    before = _books(c, [a, b])
+
+    def fail(*args, **kw):
+        raise (Stop if where == "interrupt" else RuntimeError)("planted")
+    for counts in ([1, 1], [20, 1], [2, 25]):
+        tokens = torch.cat([tok[30:30 + n] for n in counts])
+        with monkeypatch.context() as m:
+            if where == "token":
+                tokens[0] = 10 ** 6
+            elif where == "copy":
+                m.setattr(cache_module.F, "copy_pages", fail)
+            elif where == "batch":
+                m.setattr(cache_module.PagedBatch, "__init__", fail)
+            else:
+                m.setattr(model.blocks[0 if where == "first layer" else -1], "extend", fail)
+            with pytest.raises(Stop if where == "interrupt" else (RuntimeError, IndexError)):
+                model.extend(tokens, c, [a, b], counts)
+        assert _books(c, [a, b]) == before
+    out = model.extend(torch.cat([tok[30:37], tok[30:33]]), c, [a, b], [7, 3])
+    # fp32 sums of a few hundred terms in another order
+    for got, want in zip(out, (full[36], full[32])):
+        assert (got - want).abs().max() <= 2.0 ** -24 * 300 * (want.abs().max() + 1)
+
+
+def test_an_extension_can_be_taken_back():
+    c = PagedCache(1, 1, 8, 6, device="cpu", page_size=16)
+    a = c.new()
+    c.extend([a], [20])
+    b = c.fork(a)
+    before = _books(c, [a, b])
+    for counts in ([1, 1], [13, 0], [0, 30]):
+        batch = c.extend([a, b], counts)
+        assert _books(c, [a, b]) != before
+        c.take_back(batch)
+        assert _books(c, [a, b]) == before
+        c.take_back(batch)               # once only
+        assert _books(c, [a, b]) == before

@@ -64,3 +64,30 @@ def test_large_scales(scale, factor, dtype, hq, hkv, D):
             got = call().double()
             assert _code() == 0
             assert ((got - want).abs() <= bound).all(), f"{(got.isnan()).sum().item()} NaN of {got.numel()}"
+
+
+@pytest.mark.parametrize("kind", ["llama", "gpt2"])
+def test_a_failed_step_is_taken_back(kind):
+    """A step that raises half way leaves the cache as it was: the next one gives what it gives on a cache without the failure."""
+    from incin_b200.cache import PagedCache
+    from incin_b200.models.gpt2 import GPT2, GPT2Config
+    from incin_b200.models.llama import Llama, LlamaConfig
+    model = (Llama(LlamaConfig.tiny(), seed=1) if kind == "llama" else GPT2(GPT2Config.tiny(), seed=1)).cuda().to(torch.bfloat16)
+    tok = torch.randint(0, 500, (80,), generator=torch.Generator().manual_seed(2)).cuda()
+    outs = []
+    for fail in (False, True):
+        c = PagedCache.of(model, pages=20, page_size=16)
+        a = c.new()
+        model.extend(tok[:30], c, [a], [30])
+        b = c.fork(a)
+        if fail:
+            block, real = model.blocks[1], model.blocks[1].extend
+            block.extend = lambda *args: (real(*args), torch.empty(1 << 62))[0]       # out of memory behind the attention
+            for tokens, counts in ((tok[30:70], [30, 10]), (tok[30:32], None)):
+                with pytest.raises(RuntimeError):
+                    model.extend(tokens, c, [a, b], counts)
+            del block.extend
+            assert c.length(a) == c.length(b) == 30
+        outs.append(model.extend(tok[30:40], c, [a, b], [7, 3]))
+        assert _code() == 0
+    assert torch.equal(*outs)
