@@ -71,11 +71,15 @@ __device__ __forceinline__ int paged_page(const PagedView& c, int s, int i) {
   flag_bad_index(c.status);
   return -1;
 }
+// WEIGHT_LOG2: attention's weights are held as 2^WEIGHT_LOG2 at a row's reference, which the largest score may pass by 2^8.  fp16
+// has 2^16 above 1 and loses what is below 2^-25, which a long cache has much of, so the range above is used, too.
 struct Bf16 {
+  static constexpr float WEIGHT_LOG2 = 0.f;
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return unpack_bf16x2(u); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 struct Fp16 {
+  static constexpr float WEIGHT_LOG2 = 7.f;
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);

@@ -361,8 +361,9 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
           }
         }
         const float r0 = m[t][0] == -CUDART_INF_F ? 0.f : m[t][0], r1 = m[t][1] == -CUDART_INF_F ? 0.f : m[t][1];
-        float w[4] = {exp2f((s[t][0] - r0) * p.scale_log2), exp2f((s[t][1] - r1) * p.scale_log2), exp2f((s[t][2] - r0) * p.scale_log2),
-                      exp2f((s[t][3] - r1) * p.scale_log2)};
+        float w[4] = {s[t][0] - r0, s[t][1] - r1, s[t][2] - r0, s[t][3] - r1};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = exp2f(fmaf(w[e], p.scale_log2, T::WEIGHT_LOG2));
         if (key + 16 > key_end) {   // (-inf times a scale of 0 is no number)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -370,7 +371,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, NT>::CTAS_PER_SM) de
         }
         l[t][0] += w[0] + w[2];
         l[t][1] += w[1] + w[3];
-        // P in the cache's type, as the instruction wants it: half a step of relative error a weight
+        // P in the cache's type, as the instruction wants it: half a step of relative error a weight, where fp16 has normal
+        // numbers (from 2^-21 of the reference on; below, half a step of those, 2^-32 of the reference).  l sums the unrounded ones.
         pb[t][0] = transpose8x8(T::pack(w[0], w[1]));
         pb[t][1] = transpose8x8(T::pack(w[2], w[3]));
       }

@@ -559,7 +559,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int limit = it.pos0 + (live_row ? mine : min(first_token, it.tokens - 1));   // the last key that the row sees
       const int all_see = it.pos0 + first_token;                 // ... and the last one that every row of the tile sees
       float m_ref = -CUDART_INF_F;   // a score before its scale
-      float bias = 0.f;              // -scale m_ref, or 0 where it is taken off the scores themselves
+      float bias = T::WEIGHT_LOG2;   // less scale m_ref, where that is not taken off the scores themselves
       bool far = false;              // ... which the whole warp does when the reference of one of its rows is far from 0
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       for (int j = lo; j < hi; ++j) {
@@ -595,7 +595,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           const float ref = m_ref == -CUDART_INF_F ? 0.f : m_ref;   // a row that has only seen scores of -inf weighs them 0
           // (rows that hold no query have no say: what is in them changes from call to call)
           far = __any_sync(0xffffffffu, live_row && !(fabsf(ref * p.scale_log2) <= PR_FAR));
-          bias = far ? 0.f : -ref * p.scale_log2;
+          bias = far ? T::WEIGHT_LOG2 : T::WEIGHT_LOG2 - ref * p.scale_log2;
           if (far) {
 #pragma unroll
             for (int e = 0; e < PR_BM; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) - ref);
@@ -617,7 +617,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
           }
         }
-        // P in the cache's type over the first half of S_w's columns, row sums in fp32
+        // P in the cache's type over the first half of S_w's columns (half a step of relative error a weight; fp16 below 2^-21 of
+        // the reference half a step of that, 2^-32), sums of the unrounded weights in fp32
         const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(bias, bias);
 #pragma unroll
         for (int ch = 0; ch < PR_BM / 32; ++ch) {

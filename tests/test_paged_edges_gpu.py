@@ -91,3 +91,36 @@ def test_a_failed_step_is_taken_back(kind):
         outs.append(model.extend(tok[30:40], c, [a, b], [7, 3]))
         assert _code() == 0
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("place", ["first", "middle", "last"])
+@pytest.mark.parametrize("bits", [24.5, 25.5, 30.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_weights_in_fp16(place, bits, D):
+    """One key outweighs every other by 2^bits; the sum of the others' weights is still right.  fp16 keeps a weight within 2^-25
+    below 2^-14 and P is held as 2^7 at a row's reference, which is at most 2^8 off the largest score: 2^-32 a key is lost at
+    most, 2^-11 of a weight above that range."""
+    n, hkv, rows = 16384, 4, 64
+    k, v, table, _ = make_cache([n], hkv, 64, D, torch.float16, "cuda", poison=False)
+    k.zero_()
+    v.fill_(1.0)
+    at = {"first": 0, "middle": n // 2 + 5, "last": n - 1 - rows}[place]
+    z = torch.tensor(bits * 0.6931471805599453, dtype=torch.float16)
+    k[table[0, at // 64].long(), :, at % 64, 0] = z.cuda()
+    v[table[0, at // 64].long(), :, at % 64] = 0.0
+    weight = float(torch.exp(-z.double()))
+    q = torch.zeros(rows, 2 * hkv, D, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+
+    def check(out, seen):
+        tail = (seen - 1) * weight
+        want = tail / (1 + tail)
+        # half a step of the result and of each weight, exponentials and sums of 32 bits, what is lost of each weight
+        bound = want * (2 * 2.0 ** -11 + 2.0 ** -14) + seen * 2.0 ** -32
+        assert _code() == 0
+        err = (out.double().cpu() - want[:, None, None]).abs()
+        assert (err <= bound[:, None, None]).all(), f"{err.max().item():.3e} of {want[-1].item():.3e}"
+
+    lens = _i32(*[n] * rows)
+    check(_F().decode_attention(q, k, v, table.expand(rows, -1), lens, scale=1.0), torch.full((rows,), float(n)))
+    check(_F().prompt_attention(q, k, v, table, lens[:1], _i32(0, rows), scale=1.0), torch.arange(n - rows + 1, n + 1).double())
