@@ -12,7 +12,7 @@ On CUDA the tensors are bf16 or fp16 with head_dim 64 or 128, else the call is r
 entry of ``table`` that names no page, or a length that the table cannot hold, raises on the CPU; on CUDA it is met on the
 device: the entry reads as zeros, is not written through, and ``ops.gemm.check_status`` raises.
 
-None of these operators has a backward pass: they refuse inputs that want a gradient.  :class:`incin_b200.cache.PagedCache`
+None of these operators has a backward pass: they refuse inputs that want a gradient, forward-mode tangents included.  :class:`incin_b200.cache.PagedCache`
 keeps the tables.
 """
 from __future__ import annotations
@@ -22,6 +22,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 from .gemm import status_word
@@ -50,6 +51,13 @@ _KIND = {torch.bfloat16: nat.GEMM_IN_BF16, torch.float16: nat.GEMM_IN_FP16}
 # ------------------------------------------------------------------------------------------------------------- checks
 def _not_int_row(what: str, name: str, t):
     return ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
+
+
+def _no_gradient(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass and no forward-mode tangents either: call it with the primal tensors")
 
 
 def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n_heads: int):
@@ -90,8 +98,8 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
             raise _not_int_row(what, "offsets", offsets)
         if offsets.get_device() != at:
             raise ValueError(f"{what}: offsets on {offsets.device}, the others on {x.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if x.requires_grad or k_pages.requires_grad or v_pages.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient(what, x, k_pages, v_pages)
     kind = _KIND.get(dtype, -1)
     dims = (width, seqs, rows, pages, size, n_heads, hkv, D, kind)
     if at < 0:
@@ -221,8 +229,8 @@ def copy_pages(storage, src, dst):
         raise ValueError(f"copy_pages: src and dst must be int32 [pairs], got {tuple(src.shape)} {src.dtype} and {tuple(dst.shape)} {dst.dtype}")
     if src.get_device() != at or dst.get_device() != at:
         raise ValueError(f"copy_pages: tensors on {storage.device}, {src.device} and {dst.device}")
-    if torch.is_grad_enabled() and storage.requires_grad:
-        raise RuntimeError("copy_pages has no backward pass: call it under torch.no_grad()")
+    if storage.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient("copy_pages", storage)
     *outer, pages, heads, size, D = shape
     page_bytes = heads * size * D * storage.element_size()
     outer = math.prod(outer)

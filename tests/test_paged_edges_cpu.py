@@ -4,6 +4,7 @@ import torch
 
 from incin_b200.cache import PagedCache
 from incin_b200.ops import functional as F
+from incin_b200.ops import functional as F
 
 
 def _i32(*v):
@@ -75,3 +76,25 @@ def test_an_extension_can_be_taken_back():
         assert _books(c, [a, b]) == before
         c.take_back(batch)               # once only
         assert _books(c, [a, b]) == before
+
+
+def test_forward_mode_is_refused():
+    """A tangent is refused like an input that wants a gradient, by every operator and for every floating input."""
+    import torch.autograd.forward_ad as fw
+    k, v = torch.randn(4, 2, 16, 16), torch.randn(4, 2, 16, 16)
+    table, lens, off = _i32(0, 1, 2, 3).view(2, 2), _i32(20, 3), _i32(0, 1, 2)
+    q, x = torch.randn(2, 4, 16), torch.randn(2, 8 * 16)
+    want = F.decode_attention(q, k, v, table, lens)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        calls = [lambda: F.decode_attention(dual(q), k, v, table, lens), lambda: F.decode_attention(q, dual(k), v, table, lens),
+                 lambda: F.prompt_attention(q, k, dual(v), table, lens, off), lambda: F.kv_append(dual(x), k, v, table, lens, n_heads=4),
+                 lambda: F.kv_append(x, k, dual(v), table, lens, n_heads=4), lambda: F.copy_pages(dual(k), _i32(0), _i32(1))]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no backward pass"):
+                call()
+        assert torch.equal(F.decode_attention(q, k, v, table, lens), want)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        torch.func.jvp(lambda t: F.decode_attention(t, k, v, table, lens), (q,), (q,))

@@ -124,3 +124,21 @@ def test_small_weights_in_fp16(place, bits, D):
     lens = _i32(*[n] * rows)
     check(_F().decode_attention(q, k, v, table.expand(rows, -1), lens, scale=1.0), torch.full((rows,), float(n)))
     check(_F().prompt_attention(q, k, v, table, lens[:1], _i32(0, rows), scale=1.0), torch.arange(n - rows + 1, n + 1).double())
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost: refused like an input that wants a gradient."""
+    import torch.autograd.forward_ad as fw
+    F = _F()
+    k, v, table, lens = make_cache([20, 3], 2, 16, 64, torch.bfloat16, "cuda", poison=False)
+    q, x = _randn(2, 4, 64, dtype=torch.bfloat16), _randn(2, 8 * 64, dtype=torch.bfloat16)
+    want = F.decode_attention(q, k, v, table, lens)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for call in (lambda: F.decode_attention(dual(q), k, v, table, lens), lambda: F.prompt_attention(q, k, dual(v), table, lens, _i32(0, 1, 2)),
+                     lambda: F.kv_append(dual(x), k, v, table, lens, n_heads=4), lambda: F.copy_pages(dual(k)[None], _i32(0), _i32(1))):
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                call()
+        assert torch.equal(F.decode_attention(q, k, v, table, lens), want)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        torch.func.jvp(lambda t: F.decode_attention(t, k, v, table, lens), (q,), (q,))
