@@ -23,6 +23,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .. import _native as nat
 from .gemm import status_word
@@ -163,8 +164,10 @@ def kv_append(qkv, k_pages, v_pages, table, lengths, offsets=None, *, n_heads: i
     if one != 1 or step % 8 or step <= 0 or x_at % 16:   # the kernel wants dense heads on 16-byte boundaries
         qkv, step = qkv.clone(memory_format=torch.contiguous_format), wide
         x_at = qkv.data_ptr()
-    return _launch(nat.cuda().incin_kv_append, "kv_append", dims, t_row, qkv, x_at, step, D, k_pages, v_pages, table, lengths, offsets, q,
-                   args=(theta or 0.0,))
+    _launch(nat.cuda().incin_kv_append, "kv_append", dims, t_row, qkv, x_at, step, D, k_pages, v_pages, table, lengths, offsets, q,
+            args=(theta or 0.0,))
+    increment_version((k_pages, v_pages))   # written in place, for autograd's knowledge
+    return q
 
 
 # ---------------------------------------------------------------------------------------------------------- attention
@@ -260,6 +263,7 @@ def copy_pages(storage, src, dst):
         src, dst = src.contiguous(), dst.contiguous()
     nat.check(nat.cuda().incin_copy_pages(ptr, src.data_ptr(), dst.data_ptr(), n, outer, pages, page_bytes,
                                           status_word(storage.device).data_ptr(), nat.stream_ptr()), "copy_pages")
+    increment_version(storage)
     return storage
 
 

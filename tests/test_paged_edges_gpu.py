@@ -142,3 +142,22 @@ def test_forward_mode_is_refused():
         assert torch.equal(F.decode_attention(q, k, v, table, lens), want)
     with pytest.raises(RuntimeError, match="no backward pass"):
         torch.func.jvp(lambda t: F.decode_attention(t, k, v, table, lens), (q,), (q,))
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    """A value saved for a backward pass, written by an append or a page copy before that pass runs, is an error there."""
+    F = _F()
+    k, v, table, lens = make_cache([20, 3], 2, 16, 64, torch.bfloat16, "cuda", poison=False)
+    x = _randn(2, 8 * 64, dtype=torch.bfloat16)
+    for t, write in ((k, lambda: F.kv_append(x, k, v, table, lens, n_heads=4)), (v, lambda: F.kv_append(x, k, v, table, lens, n_heads=4)),
+                     (k, lambda: F.copy_pages(k[None], _i32(0), _i32(1)))):
+        w = torch.ones_like(t, requires_grad=True)
+        loss = (w * t).sum()
+        write()
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        held = torch.zeros_like(k)
+    F.kv_append(x, held, held.clone(), table, lens, n_heads=4)       # tensors without a counter are written all the same
+    F.copy_pages(held[None], _i32(0), _i32(1))
+    assert _code() == 0
