@@ -98,3 +98,12 @@ def test_forward_mode_is_refused():
         assert torch.equal(F.decode_attention(q, k, v, table, lens), want)
     with pytest.raises(RuntimeError, match="no backward pass"):
         torch.func.jvp(lambda t: F.decode_attention(t, k, v, table, lens), (q,), (q,))
+
+
+def test_copy_pages_own_copy_is_a_source_too():
+    page = lambda *v: torch.tensor(v, dtype=torch.float32).view(-1, 1, 1, 1).expand(-1, 1, 4, 4).contiguous()
+    for src, dst, want in (((0, 0), (0, 1), (0, 0, 2)), ((1, 1, 1), (2, 1, 0), (1, 1, 1))):
+        assert torch.equal(F.copy_pages(page(0, 1, 2), _i32(*src), _i32(*dst)), page(*want))
+    for src, dst in (((0, 1), (1, 1)), ((1, 0), (1, 1))):
+        with pytest.raises(IndexError):
+            F.copy_pages(page(0, 1, 2), _i32(*src), _i32(*dst))

@@ -161,3 +161,22 @@ def test_writes_in_place_are_seen_by_autograd():
     F.kv_append(x, held, held.clone(), table, lens, n_heads=4)       # tensors without a counter are written all the same
     F.copy_pages(held[None], _i32(0), _i32(1))
     assert _code() == 0
+
+
+def _pages(n=8):
+    return torch.arange(n, device="cuda", dtype=torch.float32).view(n, 1, 1, 1).expand(n, 1, 4, 4).contiguous()
+
+
+def test_copy_pages_own_copy_is_a_source_too():
+    """A page that is its own copy may be others' source, as on the CPU."""
+    for src, dst in (((0, 0), (0, 1)), ((0, 0, 3), (1, 0, 2)), ((4, 4, 4), (4, 5, 6))):
+        st, cpu = _pages(), _pages().cpu()
+        _F().copy_pages(st, _i32(*src), _i32(*dst))
+        assert _code() == 0
+        assert torch.equal(st.cpu(), _F().copy_pages(cpu, torch.tensor(src, dtype=torch.int32), torch.tensor(dst, dtype=torch.int32)))
+    for src, dst, kept in (((3, 5), (5, 5), [5]), ((5, 3), (5, 5), [5])):      # ... but not a destination, on neither
+        st = _pages()
+        _F().copy_pages(st, _i32(*src), _i32(*dst))
+        assert _code() == 6 and torch.equal(st, _pages())
+        with pytest.raises(IndexError):
+            _F().copy_pages(_pages().cpu(), torch.tensor(src, dtype=torch.int32), torch.tensor(dst, dtype=torch.int32))
