@@ -276,8 +276,8 @@ long long incin_prompt_attention_workspace(const incin_paged_desc* desc);
 int incin_prompt_attention(const incin_paged_desc* desc, void* stream);
 /* storage: `outer` runs of `pages` pages of page_bytes (a multiple of 16) each; page dst[i] becomes a copy of page src[i]
  * in every run.  A pair with an index outside [0, pages), or whose destination is an earlier pair's destination or any
- * other pair's source, is left out and reported through *status (KernelStatus 6); dst[i] == src[i] copies nothing, and may be
- * other pairs' source. */
+ * other pair's source, is left out and reported through *status (KernelStatus 6); pairs with an index outside exclude no
+ * others.  dst[i] == src[i] copies nothing, and may be other pairs' source. */
 int incin_copy_pages(void* storage, const int32_t* src, const int32_t* dst, int pairs, long long outer, int pages,
                      long long page_bytes, void* status, void* stream);
 

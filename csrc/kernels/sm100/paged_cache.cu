@@ -118,7 +118,10 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(uint4* storage
   for (int i = blockIdx.y; i < pairs; i += gridDim.y) {
     const int from = src[i], to = dst[i];
     bool bad = (unsigned)from >= (unsigned)pages || (unsigned)to >= (unsigned)pages;
-    for (int j = threadIdx.x; j < pairs; j += COPY_THREADS) bad |= j != i && ((src[j] == to && from != to) || (j < i && dst[j] == to));
+    for (int j = threadIdx.x; j < pairs; j += COPY_THREADS) {
+      if (j == i || !((src[j] == to && from != to) || (j < i && dst[j] == to))) continue;
+      bad |= (unsigned)src[j] < (unsigned)pages && (unsigned)dst[j] < (unsigned)pages;   // a pair that names no page excludes none
+    }
     if (__syncthreads_or(bad)) {
       if (threadIdx.x == 0) flag_bad_index(status);
       continue;

@@ -223,7 +223,7 @@ def copy_pages(storage, src, dst):
     type whose pages are multiples of 16 bytes; ``src``, ``dst``: int32 ``[pairs]`` on its device.  A source may be named many
     times; a destination must be named once and be nobody's source (a page may be its own copy, and others' source then).
     Pairs that break this, or name no page, raise on the CPU; on CUDA they are left out and reported through
-    ``ops.gemm.check_status``, the earliest of several equal destinations being kept."""
+    ``ops.gemm.check_status``, the earliest of several equal destinations (of pairs that name pages) being kept."""
     shape, pairs, at = storage.shape, src.shape, storage.get_device()
     if len(shape) < 4 or not storage.is_contiguous():
         raise ValueError(f"copy_pages: storage must be dense [..., pages, kv_heads, page_size, head_dim], got {tuple(shape)}, "

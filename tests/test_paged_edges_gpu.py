@@ -180,3 +180,11 @@ def test_copy_pages_own_copy_is_a_source_too():
         assert _code() == 6 and torch.equal(st, _pages())
         with pytest.raises(IndexError):
             _F().copy_pages(_pages().cpu(), torch.tensor(src, dtype=torch.int32), torch.tensor(dst, dtype=torch.int32))
+
+
+def test_copy_pages_pairs_that_name_no_page_exclude_no_other():
+    for src, dst, want in (((-1, 2), (5, 5), [0, 1, 2, 3, 4, 2, 6, 7]), ((2, 8, 3), (5, 5, 5), [0, 1, 2, 3, 4, 2, 6, 7]),
+                           ((5, 3), (8, 5), [0, 1, 2, 3, 4, 3, 6, 7]), ((5, 3, 1), (-2, 5, 5), [0, 1, 2, 3, 4, 3, 6, 7])):
+        st = _pages()
+        _F().copy_pages(st, _i32(*src), _i32(*dst))
+        assert _code() == 6 and st[:, 0, 0, 0].tolist() == want
