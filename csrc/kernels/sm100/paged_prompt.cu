@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PrParams p) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const float f = __shfl_sync(0xffffffffu, weight, (i0 + u) & 31);
-      if (i0 + u < p.splits && f != 0.f) {   // a part without weight was not written
+      if (i0 + u < p.splits) {   // one without weight, too: 0 times a value that is not finite is not 0
 #pragma unroll
         for (int e = 0; e < PER; ++e) acc[e] += f * part[u][e];
       }

@@ -188,3 +188,23 @@ def test_copy_pages_pairs_that_name_no_page_exclude_no_other():
         st = _pages()
         _F().copy_pages(st, _i32(*src), _i32(*dst))
         assert _code() == 6 and st[:, 0, 0, 0].tolist() == want
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_non_finite_values_of_small_weight(bad, D):
+    """A non-finite value that every row sees makes its element non-finite, however small its weight and wherever the keys are
+    split: 0 times it is no number either."""
+    new, past, hq, hkv = [40], [9000], 6, 2
+    k, v, table, lens = make_cache([9040], hkv, 64, D, torch.bfloat16, "cuda", poison=False)
+    q = torch.zeros(40, hq, D, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1.0
+    k.zero_()
+    for at in (5, 4000, 8000):
+        kk, vv = k.clone(), v.clone()
+        kk[table[0, 8990 // 64].long(), :, 8990 % 64, 0] = 1000.0       # outweighs all others by e^1000
+        vv[table[0, at // 64].long(), 0, at % 64, 3] = bad
+        for out in (_F().prompt_attention(q, kk, vv, table, lens, _i32(0, 40), scale=1.0), _F().decode_attention(q[:1], kk, vv, table, lens, scale=1.0)):
+            odd = ~torch.isfinite(out)
+            assert odd[:, :3, 3].all() and not odd[:, 3:].any() and odd.sum() == 3 * out.shape[0]
+    assert _code() == 0
