@@ -246,8 +246,8 @@ int incin_flash_attn_bwd(const incin_attn_desc* desc, void* stream);
  * lengths[s] counts the tokens of the sequence with its new ones.  The new tokens of all sequences are packed rows:
  * sequence s has rows [offsets[s], offsets[s + 1]), its last row is its last token; offsets == NULL: one row a sequence.
  * table, lengths and offsets are read on the device, so a captured launch follows their contents.  A length beyond the
- * table or an entry outside [0, pages) that is met writes KernelStatus 6 to *status; the entry reads as zeros and is not
- * written through.  Outputs of rows outside every sequence, and of sequences without tokens, are zeros.
+ * table, offsets that fall or lie outside [0, rows] or an entry outside [0, pages) that is met write KernelStatus 6 to *status;
+ * the entry reads as zeros and is not written through.  Outputs of rows outside every sequence, and of sequences without tokens, are zeros.
  * Hq is a multiple of Hkv, Hq / Hkv at most 128.  A table holds up to 2^30 tokens a sequence; decode wants token strides
  * below 2^23 elements.  scale (of attention only) lies in [0, 1e38]. */
 typedef struct incin_paged_desc {

@@ -64,6 +64,8 @@ __device__ __forceinline__ int paged_length(const PagedView& c, int s) {
   }
   return n;
 }
+// Whether the rows [a, b) of a sequence fall or lie outside the rows there are.
+__device__ __forceinline__ bool bad_offsets(const PagedView& c, int a, int b) { return a < 0 || b < a || b > c.rows; }
 // Page of entry i of sequence s, or -1 (and a report) when the entry names none.
 __device__ __forceinline__ int paged_page(const PagedView& c, int s, int i) {
   const int page = c.table[s * c.table_stride + i];

@@ -62,6 +62,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const PagedView c, const
       pos_of[threadIdx.x] = pos;
       page_of[threadIdx.x] = page;
     }
+  } else if (blockIdx.x == 0 && c.offsets) {   // once a launch, beside the chain above
+    for (int s = threadIdx.x - 32; s < c.seqs; s += 256 - 32)
+      if (bad_offsets(c, c.offsets[s], c.offsets[s + 1])) flag_bad_index(c.status);
   }
   __syncthreads();
   if (rotate) {

@@ -242,10 +242,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           const int s = chunk + lane;
           my_items = my_pairs = my_row = my_new = my_len = 0;
           if (s < c.seqs) {
-            my_row = min(max(c.offsets[s], 0), c.rows);
-            my_new = min(max(c.offsets[s + 1], my_row), c.rows) - my_row;
+            const int a = c.offsets[s], b = c.offsets[s + 1];
+            my_row = min(max(a, 0), c.rows);
+            my_new = min(max(b, my_row), c.rows) - my_row;
             my_len = paged_length(c, s);
-            if (my_new > my_len) flag_bad_index(c.status);
+            if (my_new > my_len || bad_offsets(c, a, b)) flag_bad_index(c.status);
             my_pairs = (my_new * group + item_rows - 1) / item_rows;
             my_items = my_pairs * per;
           }

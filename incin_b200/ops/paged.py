@@ -9,8 +9,9 @@ are int32 tensors that are read on the device: no call synchronises, and a captu
 tokens, give zeros.
 
 On CUDA the tensors are bf16 or fp16 with head_dim 64 or 128, else the call is refused; the CPU takes any float type.  An
-entry of ``table`` that names no page, or a length that the table cannot hold, raises on the CPU; on CUDA it is met on the
-device: the entry reads as zeros, is not written through, and ``ops.gemm.check_status`` raises.
+entry of ``table`` that names no page, a length that the table cannot hold, or offsets that fall or lie outside the rows raise
+on the CPU; on CUDA they are met on the device: the entry reads as zeros, is not written through, and
+``ops.gemm.check_status`` raises.
 
 None of these operators has a backward pass: they refuse inputs that want a gradient, forward-mode tangents included.  :class:`incin_b200.cache.PagedCache`
 keeps the tables.

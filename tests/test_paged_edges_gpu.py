@@ -208,3 +208,23 @@ def test_non_finite_values_of_small_weight(bad, D):
             odd = ~torch.isfinite(out)
             assert odd[:, :3, 3].all() and not odd[:, 3:].any() and odd.sum() == 3 * out.shape[0]
     assert _code() == 0
+
+
+@pytest.mark.parametrize("seqs", [3, 70])
+def test_offsets_outside_the_rows_are_reported(seqs):
+    """Offsets that fall, are negative or pass the rows: reported by both operators that read them, wherever in a batch."""
+    F = _F()
+    hq, hkv, D, rows = 4, 2, 64, 30
+    k, v, table, lens = make_cache([70] * seqs, hkv, 16, D, torch.bfloat16, "cuda", poison=False)
+    q, x = _randn(rows, hq, D, dtype=torch.bfloat16), _randn(rows, (hq + 2 * hkv) * D, dtype=torch.bfloat16)
+    cuts = sorted(min(i, rows) for i in range(seqs + 1))
+    for at, value, code in ((0, 0, 0), (seqs, rows, 0), (seqs, rows + 1, 6), (seqs, 2 ** 31 - 1, 6), (0, -1, 6), (0, -2 ** 31, 6), (seqs, 0, 6),
+                            (1, rows + 5, 6), (seqs - 1, -7, 6)):
+        offs = list(cuts)
+        offs[at] = value
+        good = all(0 <= a <= b <= rows for a, b in zip(offs, offs[1:]))
+        assert good == (code == 0)
+        F.prompt_attention(q, k, v, table, lens, _i32(*offs))
+        assert _code() == code, f"prompt_attention: offsets[{at}] = {value}"
+        F.kv_append(x, k.clone(), v.clone(), table, lens, _i32(*offs), n_heads=hq)
+        assert _code() == code, f"kv_append: offsets[{at}] = {value}"
