@@ -247,7 +247,7 @@ def copy_pages(storage, src, dst):
             raise IndexError(f"copy_pages: page outside [0, {pages})")
         if len(set(b)) != len(b) or any(j in a for _, j in moves):
             raise IndexError("copy_pages: a destination is named twice or is also a source")
-        if moves:
+        if moves and storage.numel():
             flat = storage.view(outer, pages, -1)
             flat[:, [j for _, j in moves]] = flat[:, [i for i, _ in moves]]
         return storage

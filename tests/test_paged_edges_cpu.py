@@ -107,3 +107,12 @@ def test_copy_pages_own_copy_is_a_source_too():
     for src, dst in (((0, 1), (1, 1)), ((1, 0), (1, 1))):
         with pytest.raises(IndexError):
             F.copy_pages(page(0, 1, 2), _i32(*src), _i32(*dst))
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 1, 16, 16), (3, 0, 4, 1, 16, 16), (2, 4, 0, 16, 16), (2, 4, 1, 16, 0)])
+def test_copy_pages_of_nothing(shape):
+    """No layers, or pages without elements: nothing to copy, and the pairs are looked at all the same."""
+    st = torch.zeros(shape)
+    assert F.copy_pages(st, _i32(0, 1), _i32(2, 3)) is st
+    with pytest.raises(IndexError):
+        F.copy_pages(st, _i32(0), _i32(4))
