@@ -23,7 +23,7 @@ from dataclasses import dataclass, field
 import torch
 
 from .ops import functional as F
-from .ops.paged import PAGE_SIZES
+from .ops.paged import PAGE_SIZES, check_kernels
 
 
 class CacheFull(RuntimeError):
@@ -94,10 +94,13 @@ class PagedCache:
 
     @classmethod
     def of(cls, model, pages: int, *, page_size: int = 64) -> "PagedCache":
-        """A cache for ``model`` (``models.Llama`` or ``models.GPT2``), in its parameters' type and on their device."""
+        """A cache for ``model`` (``models.Llama`` or ``models.GPT2``), in its parameters' type and on their device.  Refused where
+        the operators have no kernels for it: on CUDA they take bf16 and fp16 with head_dim 64 or 128."""
         cfg, p = model.cfg, next(model.parameters())
         heads = getattr(cfg, "n_kv_head", cfg.n_head)
         head_dim = getattr(cfg, "head_dim", cfg.d_model // cfg.n_head)
+        if p.is_cuda:
+            check_kernels("PagedCache", p.dtype, head_dim, cfg.n_head // heads)
         return cls(cfg.n_layer, heads, head_dim, pages, page_size=page_size, dtype=p.dtype, device=p.device)
 
     # ------------------------------------------------------------------------------------------------ what is in it

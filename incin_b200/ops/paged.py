@@ -55,6 +55,14 @@ def _not_int_row(what: str, name: str, t):
     return ValueError(f"{what}: {name} must be int32 with contiguous rows, got {t.dtype}, strides {t.stride()}")
 
 
+def check_kernels(what: str, dtype: torch.dtype, head_dim: int, group: int) -> None:
+    """Raises where CUDA has no kernels for such a cache; ``group``: query heads of a key head."""
+    if dtype not in _KIND or (head_dim != 64 and head_dim != 128):
+        raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {head_dim} (bf16 or fp16, head_dim 64 or 128)")
+    if group > 128:
+        raise nat.NativeError(f"{what}: {group} query heads share a key head (at most 128)")
+
+
 def _no_gradient(what: str, *tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
@@ -106,10 +114,7 @@ def _check(what: str, x, k_pages, v_pages, table, lengths, offsets, rows: int, n
     dims = (width, seqs, rows, pages, size, n_heads, hkv, D, kind)
     if at < 0:
         return at, dims, t_row
-    if kind < 0 or (D != 64 and D != 128):
-        raise nat.NativeError(f"{what}: no kernel for {dtype} with head_dim {D} (bf16 or fp16, head_dim 64 or 128)")
-    if n_heads // hkv > 128:
-        raise nat.NativeError(f"{what}: {n_heads // hkv} query heads share a key head (at most 128)")
+    check_kernels(what, dtype, D, n_heads // hkv)
     return at, dims, t_row
 
 

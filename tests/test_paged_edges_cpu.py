@@ -116,3 +116,14 @@ def test_copy_pages_of_nothing(shape):
     assert F.copy_pages(st, _i32(0, 1), _i32(2, 3)) is st
     with pytest.raises(IndexError):
         F.copy_pages(st, _i32(0), _i32(4))
+
+
+def test_what_has_kernels():
+    from incin_b200 import _native as nat
+    from incin_b200.ops.paged import check_kernels
+    for dtype in (torch.bfloat16, torch.float16):
+        for D in (64, 128):
+            check_kernels("x", dtype, D, 128)
+    for dtype, D, group in ((torch.float32, 64, 1), (torch.float64, 128, 1), (torch.bfloat16, 32, 1), (torch.float16, 256, 1), (torch.bfloat16, 64, 129)):
+        with pytest.raises(nat.NativeError, match="x: "):
+            check_kernels("x", dtype, D, group)

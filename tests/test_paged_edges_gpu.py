@@ -228,3 +228,14 @@ def test_offsets_outside_the_rows_are_reported(seqs):
         assert _code() == code, f"prompt_attention: offsets[{at}] = {value}"
         F.kv_append(x, k.clone(), v.clone(), table, lens, _i32(*offs), n_heads=hq)
         assert _code() == code, f"kv_append: offsets[{at}] = {value}"
+
+
+def test_a_cache_without_kernels_is_refused_at_once():
+    """A model whose type has no kernels on CUDA is refused when its cache is made, not by the first call."""
+    from incin_b200 import _native as nat
+    from incin_b200.cache import PagedCache
+    from incin_b200.models.llama import Llama, LlamaConfig
+    with pytest.raises(nat.NativeError, match="float32"):
+        PagedCache.of(Llama(LlamaConfig.tiny()).cuda(), pages=4)
+    PagedCache.of(Llama(LlamaConfig.tiny()).cuda().half(), pages=4)
+    PagedCache.of(Llama(LlamaConfig.tiny()), pages=4)
