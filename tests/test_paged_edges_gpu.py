@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from _paged import make_cache, tokens_of
+from _paged import attention_ref, make_cache, tokens_of
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +239,44 @@ def test_a_cache_without_kernels_is_refused_at_once():
         PagedCache.of(Llama(LlamaConfig.tiny()).cuda(), pages=4)
     PagedCache.of(Llama(LlamaConfig.tiny()).cuda().half(), pages=4)
     PagedCache.of(Llama(LlamaConfig.tiny()), pages=4)
+
+
+def test_no_wait_runs_out_for_odd_offsets():
+    """Offsets that fall, start late, pass the rows or overlap: the status word tells of them, never of a wait; rows of one
+    sequence alone are those of that run."""
+    F = _F()
+    hq, hkv, D, lengths = 4, 2, 64, [40, 50, 33]
+    k, v, table, lens = make_cache(lengths, hkv, 16, D, torch.bfloat16, "cuda", poison=False)
+    q = _randn(30, hq, D, dtype=torch.bfloat16)
+    # offsets, whether they are in order, (sequence, first row, end, rows of it that no other sequence has)
+    for offs, code, runs in (((5, 10, 20, 30), 0, [(0, 5, 10, range(5, 10)), (1, 10, 20, range(10, 20)), (2, 20, 30, range(20, 30))]),
+                             ((0, 10, 10, 500), 6, [(0, 0, 10, range(10))]), ((0, 25, 10, 30), 6, [(0, 0, 25, range(10)), (2, 10, 30, range(25, 30))]),
+                             ((-7, 3, 2 ** 31 - 1, 4), 6, []), ((30, 20, 10, 0), 6, []), ((0, 0, 0, 0), 0, [])):
+        for _ in range(3):
+            out = F.prompt_attention(q, k, v, table, lens, _i32(*offs))
+        assert _code() == code
+        for s, a, b, alone in runs:
+            want, bound = attention_ref(q[a:b], k, v, table[s:s + 1], lens[s:s + 1], _i32(0, b - a), D ** -0.5)
+            rows = torch.tensor(list(alone), device="cuda")
+            assert ((out[rows].double() - want[rows - a]).abs() <= bound[rows - a]).all()
+
+
+def test_no_wait_runs_out_for_idle_slots():
+    """A captured batch whose slots empty and fill: idle ones have a row each by the prompt's offsets, more rows than tokens,
+    which is reported as such and as nothing else."""
+    F = _F()
+    hq, hkv, D, S = 8, 2, 64, 5
+    k, v, table, lens = make_cache([600] * S, hkv, 16, D, torch.bfloat16, "cuda", poison=False)
+    q, offs = _randn(S, hq, D, dtype=torch.bfloat16), torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    F.prompt_attention(q, k, v, table, lens, offs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one, many = F.decode_attention(q, k, v, table, lens), F.prompt_attention(q, k, v, table, lens, offs)
+    for now in ([600, 1, 17, 300, 2], [0, 1, 600, 0, 0], [0] * 5, [5, 0, 0, 0, 600], [1] * 5):
+        lens.copy_(_i32(*now))
+        for _ in range(3):
+            graph.replay()
+        assert _code() == (6 if 0 in now else 0)
+        want, bound = attention_ref(q, k, v, table, lens, None, D ** -0.5)      # zeros for idle slots
+        for out in (one, many):
+            assert ((out.double() - want).abs() <= bound).all()
