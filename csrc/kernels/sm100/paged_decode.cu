@@ -2,16 +2,18 @@
 //
 //   o_h = sum_j p_hj v_j,  p_hj = 2^(c (z_hj - m_h)) / l_h,  z = q_h k_j,  c = scale log2(e),  j < lengths[b]
 //
-// Every cached key and value is used once, so the bytes of the cache bound it.  The query heads of a key head are the
-// columns of one product: S^T [16 keys x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T with m16n8k16 matrix
-// instructions (tcgen05.mma wants 128 rows; here a row of its operand would be a key that is used for 8 columns, and the
-// tiles would have to pass through shared memory).  Both operands go from global memory straight into the registers that the instructions read,
-// 16 bytes a load: the order in which a product runs over D, and in which its rows of V^T are numbered, is free, so it is
-// chosen to be the order in which the bytes arrive.  K: lane (r, c) = (lane / 4, lane % 4) loads key rows r and r + 8 at
-// element 32 j + 8 c: its four 32-bit words are the k indices of two instructions, and the queries are held in the same order.
-// V: it loads keys 2c, 2c + 1, 2c + 8, 2c + 9 at element 64 j + 8 r; a pair of keys and a word make two rows of V^T by two
-// byte permutes.  P^T comes out of S^T by transposing 8 x 8 blocks between the lanes (movmatrix).  No shared memory, no
-// barrier in the loop: a warp asks for its next keys as soon as the present ones are used, and values likewise.
+// Every cached key and value is read once for up to 16 query heads of its key head, so the bytes of the cache bound it.  (More
+// heads are dealt out in blocks of 16, each of which reads it again: 64 sequences of up to 8192, one key head of 128: 8 query
+// heads 31 us, 16 33, 32 56, 64 100, 128 187.)  The query heads of a key head are the columns of one product: S^T [16 keys x 8
+// heads] = K Q^T and O^T [D x 8 heads] += V^T P^T with m16n8k16 matrix instructions (tcgen05.mma wants 128 rows; here a row of
+// its operand would be a key that is used for 8 columns, and the tiles would have to pass through shared memory).  Both
+// operands go from global memory straight into the registers that the instructions read, 16 bytes a load: the order in which a
+// product runs over D, and in which its rows of V^T are numbered, is free, so it is chosen to be the order in which the bytes
+// arrive.  K: lane (r, c) = (lane / 4, lane % 4) loads key rows r and r + 8 at element 32 j + 8 c: its four 32-bit words are
+// the k indices of two instructions, and the queries are held in the same order. V: it loads keys 2c, 2c + 1, 2c + 8, 2c + 9 at
+// element 64 j + 8 r; a pair of keys and a word make two rows of V^T by two byte permutes.  P^T comes out of S^T by transposing
+// 8 x 8 blocks between the lanes (movmatrix).  No shared memory, no barrier in the loop: a warp asks for its next keys as soon
+// as the present ones are used, and values likewise.
 //
 // Work is dealt out by the tokens that are really there: unit = 64 tokens of one (sequence, key head), a CTA takes an equal run
 // of all units, each warp 16 tokens of every one.  Where CTAs get several units, a pair of sequence and head has one more
@@ -21,7 +23,7 @@
 // and a captured launch stays balanced whatever its lengths become.
 //
 // Bytes of the cache a second, of a measured copy's 6.47 TB/s: 128 sequences of up to 8192 tokens, 24 / 8 heads of 128, 334 us,
-// 6.7 TB/s; one of 131071, 88.7 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 87.6 us, 6.1; 64 of them 26.1 us, 4.7.  What is left
+// 6.7 TB/s; one of 131071, 88.7 us, 6.1; 256 of up to 4096, 32 / 4 heads of 64, 87.9 us, 6.1; 64 of them 26.4 us, 4.6.  What is left
 // is a chain at both ends: lengths, page numbers, first keys (4 us from the launch to the first product), and 3 us for the join.
 #include "paged.cuh"
 

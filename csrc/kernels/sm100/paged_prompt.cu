@@ -24,12 +24,13 @@
 // - A CTA takes the next item when it has done its own (clusterlaunchcontrol: it takes over a CTA of the grid that has not
 //   started).  Dealt out in advance, 16 runs of 8000 tokens in all took 119 us in place of 102, 32 / 4 heads of 64.
 //
-// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 324 us, 1.27 PFLOP/s, in short bursts, more for seconds
-// under the power cap (990 W; the dense kernel 317 and 368); 16 runs of 8000 in all, 32 / 4 heads of 64, 105 us, 0.50 (1965 MHz,
-// 840 W); 256 tokens behind 32768, 24 / 8 heads of 128, 99 us, 1.04; 37 tokens 7 us.
+// Measured, and in operations a second: one run of 8191, 24 / 8 heads of 128, 327 to 335 us in short bursts, 1.23 to 1.26 PFLOP/s,
+// 386 us, 1.07, call after call under the power cap (990 W; the dense kernel 317 and 368); 16 runs of 8000 in all, 32 / 4 heads of
+// 64, 107 and 109 us, 0.49 (1965 MHz, 840 W); 256 tokens behind 32768, 24 / 8 heads of 128, 100 and 118 us, 1.03 and 0.87; 37
+// tokens 7 us.
 // What bounds it: a K / V tile takes a pair of query tiles 1.5 to 1.6 us at either head_dim, of which the tensor pipe, the
-// special-function unit and tensor memory are each busy two thirds (ncu at head_dim 128: 63, 63 and 66 %); a warp's
-// row takes 1360-1480 clocks for its exponentials (1024 at the unit's rate), 500 for its maximum, and waits 620-930 for its scores.
+// special-function unit and tensor memory are each busy two thirds (ncu at head_dim 128: 62, 62 and 64 %); a warp's
+// row takes 1420-1650 clocks for its exponentials (1024 at the unit's rate), 470-640 for its maximum, and waits 540-990 for its scores.
 // Tried and slower, with that time in view: exponentials before the maximum is known (340 -> 355 us); the two warps of a
 // scheduler taking turns with theirs (331 -> 393 us at head_dim 64); P in columns of its own at head_dim 64 and the next scores
 // ahead of the product (331 -> 410); three regions for scores there, in turn, with the same aim (346 -> 361); masked tiles
@@ -99,7 +100,7 @@ struct PrParams {
   int tiles;           // query tiles of an item: 2, or 1 where twice as many items are wanted
   int splits;
   float* part_o;       // [splits][rows][Hq][D]
-  float2* part_ml;     // [splits][rows][Hq]: m and l; l = -1 for a row without a position, -2 in the first split of one that is done
+  float2* part_ml;     // [splits][rows][Hq]: m (a score before its scale) and l; l = -1 for a row without a position, -2 in the first split of one that is done
 };
 
 template <typename T>
@@ -771,7 +772,7 @@ struct PrPlan {
 // Query tiles of an item and CTAs that share its keys, by the time that the longest items take in all, in ns.  Measured at
 // head_dim 128 (24 / 8 heads) and 64 (32 / 4): a K / V tile takes a pair of query tiles 1580 and a single one 1460, an item's
 // beginning and end 1500, the joining kernel 3500 and its parts' bytes.  256 tokens behind 32768: single tiles and two splits
-// 214 us, pairs and four 126 us, nine 133; 500 tokens alone: single tiles 14.1 us, pairs 15.0, two splits 25.8.
+// 217 us, pairs and four 129, six (the rule's) 100, nine 128; 500 tokens alone: single tiles 13.9 us, pairs 15.0, two splits 19.5.
 static PrPlan pr_plan(const incin_paged_desc* d) {
   PrPlan pl = {};
   const int sms = device_sm_count();

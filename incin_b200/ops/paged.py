@@ -13,8 +13,12 @@ entry of ``table`` that names no page, a length that the table cannot hold, or o
 on the CPU; on CUDA they are met on the device: the entry reads as zeros, is not written through, and
 ``ops.gemm.check_status`` raises.
 
-None of these operators has a backward pass: they refuse inputs that want a gradient, forward-mode tangents included.  :class:`incin_b200.cache.PagedCache`
-keeps the tables.
+Attention rounds each weight to the tensors' type before it multiplies a value, as the dense attention does; scores, weights'
+sums and results are held in 32 bits until the end.  Against 64 bits its error is 1.2 to 1.4 times that of a form that is
+rounded once (bf16 0.0023 in place of 0.0017 of the result's norm, fp16 0.00029 in place of 0.00021).
+
+None of these operators has a backward pass: they refuse inputs that want a gradient, forward-mode tangents included.
+:class:`incin_b200.cache.PagedCache` keeps the tables.
 """
 from __future__ import annotations
 
