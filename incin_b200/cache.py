@@ -223,7 +223,7 @@ class PagedCache:
 
     def take_back(self, batch: PagedBatch) -> None:
         """Undo the :meth:`extend` that made ``batch``: lengths, pages and their owners are as before it.  For a pass that failed,
-        before anything else is done with its sequences."""
+        before anything else is done to the cache."""
         self._restore(batch._undo)
 
     def admit(self, tokens: torch.Tensor, seqs: list[int], counts: list[int] | None, max_seq: int) -> PagedBatch:
